@@ -43,6 +43,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   register_adam(m);
   register_ce(m);
   register_attn_tc(m);
+  register_attn_window(m);
   register_symm(m);
   register_tp(m);
 }

@@ -18,6 +18,11 @@ int num_sms();
 CUtensorMap make_tmap_bf16(const void* base, uint64_t inner, uint64_t outer, uint64_t ld, uint32_t box_inner,
                            uint32_t box_outer);
 
+// 4-D bf16 tensor: `dims` innermost first, `strides` in bytes of the outer
+// three (multiples of 16); 128B-swizzled box of `box`.
+CUtensorMap make_tmap_bf16_4d(const void* base, const uint64_t (&dims)[4], const uint64_t (&strides)[3],
+                              const uint32_t (&box)[4]);
+
 }  // namespace dst
 
 void register_gemm(pybind11::module& m);
@@ -26,5 +31,6 @@ void register_embed(pybind11::module& m);
 void register_adam(pybind11::module& m);
 void register_ce(pybind11::module& m);
 void register_attn_tc(pybind11::module& m);
+void register_attn_window(pybind11::module& m);
 void register_symm(pybind11::module& m);
 void register_tp(pybind11::module& m);

@@ -50,6 +50,27 @@ CUtensorMap make_tmap_bf16(const void* base, uint64_t inner, uint64_t outer, uin
   return m;
 }
 
+CUtensorMap make_tmap_bf16_4d(const void* base, const uint64_t (&dims)[4], const uint64_t (&strides)[3],
+                              const uint32_t (&box)[4]) {
+  CUtensorMap m;
+  cuuint64_t d[4], st[3];
+  cuuint32_t bx[4], estr[4] = {1, 1, 1, 1};
+  for (int i = 0; i < 4; ++i) {
+    d[i] = dims[i];
+    bx[i] = box[i];
+  }
+  TORCH_CHECK(reinterpret_cast<uintptr_t>(base) % 16 == 0, "TMA base must be 16-byte aligned");
+  for (int i = 0; i < 3; ++i) {
+    TORCH_CHECK(strides[i] % 16 == 0, "TMA strides must be multiples of 16 bytes");
+    st[i] = strides[i];
+  }
+  CUresult r = encode_fn()(&m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(base), d, st, bx, estr,
+                           CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                           CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  TORCH_CHECK(r == CUDA_SUCCESS, "cuTensorMapEncodeTiled failed: ", static_cast<int>(r));
+  return m;
+}
+
 int num_sms() {
   static int n[64] = {0};
   int dev;
