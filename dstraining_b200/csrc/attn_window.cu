@@ -697,6 +697,9 @@ __global__ void __launch_bounds__(kThreads, DqCfg<DP>::kCtas)
 // [B, T, H, D] with unit inner stride; the other strides and the base must be
 // multiples of 16 bytes (a dimension of size 1 may have any stride).
 void check_operand(const at::Tensor& x, const char* name) {
+  TORCH_CHECK(x.dim() != 4 || (x.size(3) >= 8 && x.size(3) <= 128 && x.size(3) % 8 == 0),
+              "window attention: head_dim must be a multiple of 8 up to 128, got ",
+              std::to_string(x.size(3)));
   TORCH_CHECK(x.is_cuda() && x.scalar_type() == at::kBFloat16 && x.dim() == 4, "window attention: ", name,
               " must be a CUDA bf16 tensor [B, T, H, D]");
   TORCH_CHECK(x.stride(3) == 1 && reinterpret_cast<uintptr_t>(x.data_ptr()) % 16 == 0, "window attention: ", name,
@@ -720,7 +723,6 @@ CUtensorMap map_of(const at::Tensor& x, int rows) {
 
 Shape shape_of(const at::Tensor& q, const at::Tensor& k, int64_t window, int64_t sinks) {
   const int64_t T = q.size(1), D = q.size(3);
-  TORCH_CHECK(D >= 8 && D <= 128 && D % 8 == 0, "window attention: head_dim must be a multiple of 8 up to 128, got ", D);
   TORCH_CHECK(T >= 1 && T < (int64_t(1) << 30) && q.size(0) >= 1, "window attention: T and B must be positive");
   TORCH_CHECK(q.size(2) <= 65535 && q.size(0) <= 65535, "window attention: more than 65535 heads or sequences");
   TORCH_CHECK(k.size(2) >= 1 && q.size(2) % k.size(2) == 0,

@@ -44,6 +44,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   register_ce(m);
   register_attn_tc(m);
   register_attn_window(m);
+  register_kv_cache(m);
+  register_sampling(m);
   register_symm(m);
   register_tp(m);
 }

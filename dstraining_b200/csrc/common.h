@@ -32,5 +32,7 @@ void register_adam(pybind11::module& m);
 void register_ce(pybind11::module& m);
 void register_attn_tc(pybind11::module& m);
 void register_attn_window(pybind11::module& m);
+void register_kv_cache(pybind11::module& m);
+void register_sampling(pybind11::module& m);
 void register_symm(pybind11::module& m);
 void register_tp(pybind11::module& m);

@@ -1,0 +1,1002 @@
+// The rolling key/value cache of windowed attention with sinks, in bf16 or
+// 4 bits, and the attention of one new token per sequence over it.
+//
+// Slots: S + W per (sequence, key head); token p lies in slot p while p < S and
+// in S + (p - S) % W after, so once the ring is full a new token takes the slot
+// of the one that leaves the window, and every filled slot is visible.
+//
+// 4 bits: each 32 channels of a row share a step = bf16((max - min) / 15) and
+// their least value (bf16, exact: it is one of them); a channel is stored as
+// code = clamp(rint((x - min) / step), 0, 15) and stands for min + code * step.
+// 32 channels cost 20 bytes instead of 64. A group with an infinity or NaN
+// stands for NaN.
+//
+// The single-token step reads every held row once and is bound by that traffic,
+// so it has to keep many bytes in flight and spend few instructions on them:
+//   * each warp streams tiles of keys through its own ring of shared-memory
+//     stages with bulk copies (no barriers between warps, loads far ahead);
+//   * the up to 8 query heads that share a key head are the rows of
+//     mma.m16n8k16 (one query row per head: a 128-row tcgen05 tile would be
+//     empty for the most part, and at 8 rows the instruction is not the bound);
+//     4-bit codes become bf16 operands with one bit operation per pair (128 +
+//     code is exact in bf16), the steps and least values are applied to the fp32
+//     scores and to the probabilities, never to rounded keys or values;
+//   * probabilities enter the second product as the sum of two bf16 numbers in
+//     the unused rows 8..15 (relative error 2^-17), so the result carries the
+//     precision of fp32 probabilities.
+// A long cache is split over CTAs; the last one to finish joins the partial
+// results in the order of the splits (fixed order: no run-to-run differences).
+#include <ATen/cuda/CUDAContext.h>
+#include <c10/cuda/CUDAGuard.h>
+#include <torch/extension.h>
+
+#include "common.h"
+#include "ptx.cuh"
+
+namespace dst {
+namespace kv_cache {
+
+constexpr int kWarps = 4;
+constexpr int kThreads = 32 * kWarps;
+constexpr int kRows = 8;  // query heads per CTA
+
+// ------------------------------------------------------------ row formats
+// 8 channels of a row as one lane holds them.
+__device__ __forceinline__ void unpack8(const uint4& u, float (&x)[8]) {
+  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    x[2 * i] = __uint_as_float(w[i] << 16);
+    x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+  }
+}
+
+__device__ __forceinline__ float min_nan(float a, float b) {
+  float r;
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+
+struct Quant8 {
+  uint32_t code[8];
+  uint32_t param;  // step (low half) and least value (high half), bf16
+};
+
+// Codes of this lane's 8 channels; the 4 lanes of an aligned quad hold a group.
+// Division and rounding are the IEEE operations, so any implementation of the
+// definition gets the same codes.
+__device__ __forceinline__ Quant8 quantize8(const float (&x)[8]) {
+  float lo = x[0], hi = x[0];
+#pragma unroll
+  for (int i = 1; i < 8; ++i) {
+    lo = min_nan(lo, x[i]);
+    hi = max_nan(hi, x[i]);
+  }
+#pragma unroll
+  for (int o = 1; o < 4; o <<= 1) {
+    lo = min_nan(lo, __shfl_xor_sync(0xffffffff, lo, o));
+    hi = max_nan(hi, __shfl_xor_sync(0xffffffff, hi, o));
+  }
+  const __nv_bfloat16 step16 = __float2bfloat16_rn(__fdiv_rn(__fsub_rn(hi, lo), 15.f));
+  const __nv_bfloat16 low16 = __float2bfloat16_rn(lo);
+  const float step = __bfloat162float(step16);
+  Quant8 q;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const float c = step > 0.f ? __fdiv_rn(__fsub_rn(x[i], lo), step) : 0.f;
+    q.code[i] = static_cast<uint32_t>(fminf(fmaxf(rintf(c), 0.f), 15.f));
+  }
+  q.param = static_cast<uint32_t>(__bfloat16_as_ushort(step16)) |
+            (static_cast<uint32_t>(__bfloat16_as_ushort(low16)) << 16);
+  return q;
+}
+
+__device__ __forceinline__ float param_step(uint32_t p) { return __uint_as_float(p << 16); }
+__device__ __forceinline__ float param_low(uint32_t p) { return __uint_as_float(p & 0xffff0000u); }
+
+// Layout of a packed row of DP channels, NG = DP / 32 groups.
+//   keys:   word (t, g), t = 0..3, at 4 (t NG + g): the channels g*32 + t*8 + c;
+//           nibble c/2 + 4 (c & 1), so that (word >> 4 i) & 0x000f000f is the
+//           pair of channels 2 i, 2 i + 1
+//   values: half-word (n, g), n = 0..7, at 2 (n NG + g): channels g*32 + n*4 + j
+// Both are what one thread of the mma needs of a row, side by side.
+__device__ __forceinline__ uint32_t key_word(const uint32_t (&c)[8]) {
+  uint32_t w = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) w |= c[i] << (4 * ((i >> 1) + 4 * (i & 1)));
+  return w;
+}
+
+template <int DP>
+__device__ __forceinline__ void put_key8(uint8_t* row, int i, const uint32_t (&c)[8]) {
+  *reinterpret_cast<uint32_t*>(row + 4 * ((i & 3) * (DP / 32) + (i >> 2))) = key_word(c);
+}
+
+template <int DP>
+__device__ __forceinline__ void put_value8(uint8_t* row, int i, const uint32_t (&c)[8]) {
+  constexpr int NG = DP / 32;
+  const int g = i >> 2, n = (i & 3) * 2;
+#pragma unroll
+  for (int e = 0; e < 2; ++e)
+    *reinterpret_cast<uint16_t*>(row + 2 * ((n + e) * NG + g)) =
+        static_cast<uint16_t>(c[4 * e] | (c[4 * e + 1] << 4) | (c[4 * e + 2] << 8) | (c[4 * e + 3] << 12));
+}
+
+template <int DP>
+__device__ __forceinline__ void get_key8(const uint8_t* row, int i, uint32_t (&c)[8]) {
+  const uint32_t w = *reinterpret_cast<const uint32_t*>(row + 4 * ((i & 3) * (DP / 32) + (i >> 2)));
+#pragma unroll
+  for (int j = 0; j < 8; ++j) c[j] = (w >> (4 * ((j >> 1) + 4 * (j & 1)))) & 15u;
+}
+
+template <int DP>
+__device__ __forceinline__ void get_value8(const uint8_t* row, int i, uint32_t (&c)[8]) {
+  constexpr int NG = DP / 32;
+#pragma unroll
+  for (int e = 0; e < 2; ++e) {
+    const uint32_t w = *reinterpret_cast<const uint16_t*>(row + 2 * (((i & 3) * 2 + e) * NG + (i >> 2)));
+#pragma unroll
+    for (int j = 0; j < 4; ++j) c[4 * e + j] = (w >> (4 * j)) & 15u;
+  }
+}
+
+__device__ __forceinline__ void store8f(float* dst, const float (&x)[8]) {
+  *reinterpret_cast<float4*>(dst) = make_float4(x[0], x[1], x[2], x[3]);
+  *reinterpret_cast<float4*>(dst + 4) = make_float4(x[4], x[5], x[6], x[7]);
+}
+
+__device__ __forceinline__ void values8(const Quant8& q, float (&x)[8]) {
+  const float step = param_step(q.param), low = param_low(q.param);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) x[i] = fmaf(static_cast<float>(q.code[i]), step, low);  // the product is exact
+}
+
+// Where the cache of one operand (keys or values) lies: rows of `slots_alloc`
+// (a multiple of the tile) per (sequence, key head).
+struct Store {
+  uint8_t* rows;     // bf16 rows of DP, or packed rows of DP / 2 bytes
+  uint32_t* params;  // 4 bits: NG per row
+};
+
+struct Ring {
+  int64_t W, S;
+  int alloc;  // rows allocated per (sequence, key head)
+  __device__ __forceinline__ int64_t slot(int64_t p) const { return p < S ? p : S + (p - S) % W; }
+};
+
+struct View {  // k or v rows: element strides, unit inner stride
+  const __nv_bfloat16* p;
+  int64_t b, h, t;
+};
+
+__device__ __forceinline__ uint4 load8(const __nv_bfloat16* row, int i, int D) {
+  return i * 8 < D ? *reinterpret_cast<const uint4*>(row + i * 8) : make_uint4(0, 0, 0, 0);
+}
+
+// ------------------------------------------------------------- fill and read
+// The rows of the prompts' visible tokens into their slots. DP/8 lanes per row;
+// row i of a (sequence, head) is token i while that is a sink, then the tokens
+// of the last window.
+template <int DP, int BITS>
+__global__ void __launch_bounds__(256)
+    fill_kernel(const View k, const View v, const int64_t* __restrict__ lengths, int64_t* __restrict__ pos, Store ks,
+                Store vs, const Ring ring, int T, int rows, int Hk, int D, int* status) {
+  constexpr int L = DP / 8;
+  const int64_t r = (static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x) / L;
+  const int i = threadIdx.x % L;
+  const int b = blockIdx.z, hk = blockIdx.y >> 1;
+  const bool value = blockIdx.y & 1;
+  int64_t len = lengths ? lengths[b] : T;
+  if (len < 0 || len > T) {
+    if (threadIdx.x == 0) record_status(status, kBadArgument);
+    len = len < 0 ? 0 : T;
+  }
+  if (blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0) pos[b] = len;
+  const int64_t tail = len - ring.W > ring.S ? len - ring.W : ring.S;
+  const int64_t token = r < ring.S ? r : tail + (r - ring.S);
+  const bool there = r < rows && token < len;
+  if (!__any_sync(0xffffffff, there)) return;
+  const View& x = value ? v : k;
+  const Store& s = value ? vs : ks;
+  const int64_t row = (static_cast<int64_t>(b) * Hk + hk) * ring.alloc + (there ? ring.slot(token) : 0);
+  const uint4 u = there ? load8(x.p + b * x.b + token * x.t + hk * x.h, i, D) : make_uint4(0, 0, 0, 0);
+  if (BITS == 16) {
+    if (there) *reinterpret_cast<uint4*>(s.rows + row * (DP * 2) + i * 16) = u;
+  } else {
+    float f[8];
+    unpack8(u, f);
+    const Quant8 q = quantize8(f);
+    if (there) {
+      uint8_t* dst = s.rows + row * (DP / 2);
+      if (value)
+        put_value8<DP>(dst, i, q.code);
+      else
+        put_key8<DP>(dst, i, q.code);
+      if ((i & 3) == 0) s.params[row * (DP / 32) + (i >> 2)] = q.param;
+    }
+  }
+}
+
+// The held rows in slot order (0 where no token is): bf16, or fp32 for 4 bits.
+template <int DP, int BITS>
+__global__ void __launch_bounds__(256)
+    read_kernel(const Store ks, const Store vs, const int64_t* __restrict__ pos, void* __restrict__ ko,
+                void* __restrict__ vo, const Ring ring, int slots, int Hk, int D) {
+  constexpr int L = DP / 8;
+  const int64_t r = (static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x) / L;
+  const int i = threadIdx.x % L;
+  if (r >= slots || i * 8 >= D) return;
+  const int b = blockIdx.z, hk = blockIdx.y >> 1;
+  const bool value = blockIdx.y & 1;
+  const Store& s = value ? vs : ks;
+  const bool there = r < pos[b];
+  const int64_t bh = static_cast<int64_t>(b) * Hk + hk, row = bh * ring.alloc + r;
+  const int64_t dst = (bh * slots + r) * D + i * 8;
+  if (BITS == 16) {
+    *reinterpret_cast<uint4*>(reinterpret_cast<__nv_bfloat16*>(value ? vo : ko) + dst) =
+        there ? *reinterpret_cast<const uint4*>(s.rows + row * (DP * 2) + i * 16) : make_uint4(0, 0, 0, 0);
+  } else {
+    float f[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    if (there) {
+      Quant8 q;
+      if (value)
+        get_value8<DP>(s.rows + row * (DP / 2), i, q.code);
+      else
+        get_key8<DP>(s.rows + row * (DP / 2), i, q.code);
+      q.param = s.params[row * (DP / 32) + (i >> 2)];
+      values8(q, f);
+    }
+    store8f(reinterpret_cast<float*>(value ? vo : ko) + dst, f);
+  }
+}
+
+// ------------------------------------------------------------------- step
+__device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                         uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+  __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+  return *reinterpret_cast<uint32_t*>(&h);
+}
+
+// x and y as sums of two bf16 numbers each: hi pair, lo pair.
+__device__ __forceinline__ void split2(float x, float y, uint32_t& hi, uint32_t& lo) {
+  hi = pack2(x, y);
+  lo = pack2(x - __uint_as_float(hi << 16), y - __uint_as_float(hi & 0xffff0000u));
+}
+
+template <int DP, int BITS>
+struct StepCfg {
+  static constexpr int NG = DP / 32;
+  static constexpr int kRowBytes = BITS == 16 ? DP * 2 : DP / 2;
+  static constexpr int kParamBytes = BITS == 16 ? 0 : NG * 4;
+  // keys per stage of a warp's ring
+  static constexpr int KT = BITS == 16 ? (DP == 64 ? 32 : 16) : (DP == 64 ? 64 : 32);
+  static constexpr int kStages = BITS == 16 ? 3 : 2;
+  static constexpr int kOperand = KT * kRowBytes;  // keys or values of a stage
+  static constexpr int kStage = 2 * kOperand + 2 * KT * kParamBytes;
+  static constexpr int kRingBytes = kWarps * kStages * kStage;
+  // the new token's row, laid out like a stage of 16 keys
+  static constexpr int kNew = 2 * 16 * (kRowBytes + kParamBytes);
+  static constexpr int kJoin = kWarps * kRows * (DP + 2) * 4;  // over the ring at the end
+  static constexpr int kSmem = (kRingBytes > kJoin ? kRingBytes : kJoin) + kNew + kWarps * kStages * 8 + 16 + 1024;
+  static constexpr int kCtas = BITS == 16 ? 2 : (DP == 64 ? 4 : 3);  // per SM
+};
+
+struct StepArgs {
+  const __nv_bfloat16* q;
+  int64_t q_b, q_h;
+  View k, v;  // the new token's rows
+  const int64_t* pos;
+  Store ks, vs;
+  __nv_bfloat16* out;      // [B, H, D]
+  float *stored_k, *stored_v;  // optional [B, Hk, D]: what the new row stands for
+  float* partial;          // [B * Hk * chunks][splits][kRows][DP + 2]
+  int* arrived;            // [B * Hk * chunks], 0 between launches
+  Ring ring;
+  int slots, Hk, G, D, chunks, splits;
+  float scale_log2;
+  int* status;
+};
+
+// The warp's running result for the 8 query rows: thread (n = lane / 4, t =
+// lane % 4) holds for row n the output channels of columns 2t, 2t + 1 of each
+// 8-column tile, and the parts of l and of the constant terms that its keys add.
+template <int DP, int BITS>
+struct State {
+  static constexpr int NG = DP / 32;
+  float m, l;
+  float o[DP / 8][4];  // [tile]: 0, 1 high parts, 2, 3 low parts
+  float c[BITS == 4 ? NG : 1];  // sum of p (low - 128 step)
+};
+
+// One 16-byte chunk `c` of row `r` of a 128B-swizzled tile of 64 channels.
+__device__ __forceinline__ const uint4* swz(const uint8_t* tile, int r, int c) {
+  return reinterpret_cast<const uint4*>(tile + r * 128 + ((c ^ (r & 7)) << 4));
+}
+
+// NS subtiles of 16 keys each: keys and values at `sk`, `sv` (and their
+// parameters), `rows_in_tile` rows per swizzled tile; bit i of `valid` says
+// whether key i takes part.
+template <int DP, int BITS, int NS>
+__device__ __forceinline__ void attend(State<DP, BITS>& st, const uint32_t (&qa)[DP / 16][2], const float* qsum,
+                                       const uint8_t* sk, const uint8_t* sv, const uint32_t* pk, const uint32_t* pv,
+                                       int tile_rows, uint32_t valid, float scale_log2) {
+  constexpr int NG = DP / 32;
+  const int lane = threadIdx.x & 31, n = lane >> 2, t = lane & 3;
+  constexpr uint32_t kAll = NS == 2 ? 0xffffffffu : 0xffffu;
+  float s[2 * NS][2];  // scores of columns 2t, 2t + 1 of each 8 keys, row n
+#pragma unroll
+  for (int i = 0; i < 2 * NS; ++i) {
+    const int r = i * 8 + n;
+    if (BITS == 16) {
+      float acc[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int a = 0; a < DP / 64; ++a) {
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          const uint4 w = *swz(sk + a * tile_rows * 128, r, 2 * t + c);
+          mma16816(acc, qa[a * 4 + c * 2][0], 0u, qa[a * 4 + c * 2][1], 0u, w.x, w.y);
+          mma16816(acc, qa[a * 4 + c * 2 + 1][0], 0u, qa[a * 4 + c * 2 + 1][1], 0u, w.z, w.w);
+        }
+      }
+      s[i][0] = acc[0];
+      s[i][1] = acc[1];
+    } else {
+      uint32_t w[NG];
+      const uint8_t* p = sk + r * (DP / 2) + t * (DP / 8);
+      if (NG == 2) {
+        const uint2 u = *reinterpret_cast<const uint2*>(p);
+        w[0] = u.x, w[1] = u.y;
+      } else {
+        const uint4 u = *reinterpret_cast<const uint4*>(p);
+        w[0] = u.x, w[1] = u.y, w[NG - 2] = u.z, w[NG - 1] = u.w;
+      }
+      s[i][0] = s[i][1] = 0.f;
+#pragma unroll
+      for (int g = 0; g < NG; ++g) {
+        float acc[4] = {0.f, 0.f, 0.f, 0.f};
+        uint32_t b[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) b[j] = ((w[g] >> (4 * j)) & 0x000f000fu) | 0x43004300u;
+        mma16816(acc, qa[2 * g][0], 0u, qa[2 * g][1], 0u, b[0], b[1]);
+        mma16816(acc, qa[2 * g + 1][0], 0u, qa[2 * g + 1][1], 0u, b[2], b[3]);
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const uint32_t par = pk[(i * 8 + 2 * t + e) * NG + g];
+          const float step = param_step(par);
+          s[i][e] += fmaf(step, acc[e], fmaf(-128.f, step, param_low(par)) * qsum[g]);
+        }
+      }
+    }
+  }
+  float mx = -INFINITY;
+  if (valid != kAll) {
+#pragma unroll
+    for (int i = 0; i < 2 * NS; ++i)
+#pragma unroll
+      for (int e = 0; e < 2; ++e)
+        if (!((valid >> (i * 8 + 2 * t + e)) & 1u)) s[i][e] = -INFINITY;
+  }
+#pragma unroll
+  for (int i = 0; i < 2 * NS; ++i) mx = fmaxf(mx, fmaxf(s[i][0], s[i][1]));
+  mx = fmaxf(mx, __shfl_xor_sync(0xffffffff, mx, 1));
+  mx = fmaxf(mx, __shfl_xor_sync(0xffffffff, mx, 2)) * scale_log2;
+  // As in the prompt's kernel a row keeps its reference maximum until a tile
+  // exceeds it by 8 (in log2).
+  const bool need = mx > st.m + 8.f;
+  if (__any_sync(0xffffffff, need)) {
+    const float c = need ? exp2f(st.m - mx) : 1.f;
+    if (need) st.m = mx;
+    st.l *= c;
+#pragma unroll
+    for (int i = 0; i < DP / 8; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) st.o[i][j] *= c;
+    if (BITS == 4) {
+#pragma unroll
+      for (int g = 0; g < NG; ++g) st.c[g] *= c;
+    }
+  }
+  const float m_use = st.m == -INFINITY ? 0.f : st.m;
+#pragma unroll
+  for (int i = 0; i < 2 * NS; ++i)
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      s[i][e] = exp2f(fmaf(s[i][e], scale_log2, -m_use));
+      st.l += s[i][e];
+    }
+#pragma unroll
+  for (int u = 0; u < NS; ++u) {
+    const int r0 = u * 16 + 2 * t;  // this thread's keys: r0, r0 + 1, r0 + 8, r0 + 9
+    const uint32_t in = valid >> r0;
+    if (BITS == 16) {
+      uint32_t a0, a1, a2, a3;
+      split2(s[2 * u][0], s[2 * u][1], a0, a1);
+      split2(s[2 * u + 1][0], s[2 * u + 1][1], a2, a3);
+#pragma unroll
+      for (int a = 0; a < DP / 64; ++a) {
+        const uint8_t* tile = sv + a * tile_rows * 128;
+        uint4 x[4] = {*swz(tile, r0, n), *swz(tile, r0 + 1, n), *swz(tile, r0 + 8, n), *swz(tile, r0 + 9, n)};
+        if (valid != kAll) {  // what lies in a masked row must not meet its zero probability
+          const uint4 z = make_uint4(0, 0, 0, 0);
+          if (!(in & 1u)) x[0] = z;
+          if (!(in & 2u)) x[1] = z;
+          if (!(in & 0x100u)) x[2] = z;
+          if (!(in & 0x200u)) x[3] = z;
+        }
+        const uint32_t* w[4] = {&x[0].x, &x[1].x, &x[2].x, &x[3].x};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          mma16816(st.o[a * 8 + 2 * j], a0, a1, a2, a3, __byte_perm(w[0][j], w[1][j], 0x5410),
+                   __byte_perm(w[2][j], w[3][j], 0x5410));
+          mma16816(st.o[a * 8 + 2 * j + 1], a0, a1, a2, a3, __byte_perm(w[0][j], w[1][j], 0x7632),
+                   __byte_perm(w[2][j], w[3][j], 0x7632));
+        }
+      }
+    } else {
+      uint32_t w[4][NG / 2];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const uint8_t* p = sv + (r0 + (j & 1) + (j >> 1) * 8) * (DP / 2) + n * (DP / 16);
+        if (NG == 2) {
+          w[j][0] = *reinterpret_cast<const uint32_t*>(p);
+        } else {
+          const uint2 x = *reinterpret_cast<const uint2*>(p);
+          w[j][0] = x.x, w[j][NG / 2 - 1] = x.y;
+        }
+      }
+#pragma unroll
+      for (int g = 0; g < NG; ++g) {
+        float x[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          uint32_t par = pv[(r0 + (j & 1) + (j >> 1) * 8) * NG + g];
+          if (valid != kAll && !((in >> ((j & 1) + (j >> 1) * 8)) & 1u)) par = 0u;
+          const float p = s[2 * u + (j >> 1)][j & 1], step = param_step(par);
+          x[j] = p * step;
+          st.c[g] = fmaf(p, fmaf(-128.f, step, param_low(par)), st.c[g]);
+        }
+        uint32_t a0, a1, a2, a3;
+        split2(x[0], x[1], a0, a1);
+        split2(x[2], x[3], a2, a3);
+        const uint32_t sel = (g & 1) ? 0x7632 : 0x5410;
+        const uint32_t lo = __byte_perm(w[0][g >> 1], w[1][g >> 1], sel);
+        const uint32_t hi = __byte_perm(w[2][g >> 1], w[3][g >> 1], sel);
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          mma16816(st.o[g * 4 + j], a0, a1, a2, a3, ((lo >> (4 * j)) & 0x000f000fu) | 0x43004300u,
+                   ((hi >> (4 * j)) & 0x000f000fu) | 0x43004300u);
+      }
+    }
+  }
+}
+
+// Output channel of tile `tile`, column `n`.
+template <int DP, int BITS>
+__device__ __forceinline__ int channel_of(int tile, int n) {
+  return BITS == 16 ? (tile >> 3) * 64 + n * 8 + (tile & 7) : (tile >> 2) * 32 + n * 4 + (tile & 3);
+}
+
+template <int DP, int BITS>
+__global__ void __launch_bounds__(kThreads, StepCfg<DP, BITS>::kCtas)
+    step_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const StepArgs a) {
+  using C = StepCfg<DP, BITS>;
+  constexpr int NG = C::NG, KT = C::KT, ST = C::kStages;
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* fresh = smem + (C::kRingBytes > C::kJoin ? C::kRingBytes : C::kJoin);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(fresh + C::kNew);
+  int* last_flag = reinterpret_cast<int*>(bars + kWarps * ST);
+
+  const int split = blockIdx.x, b = blockIdx.z;
+  const int hk = blockIdx.y / a.chunks, chunk = blockIdx.y % a.chunks;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, n = lane >> 2, t = lane & 3;
+  const int heads = min(kRows, a.G - chunk * kRows);  // query heads of this CTA
+  const int h0 = hk * a.G + chunk * kRows;
+  const int64_t p = a.pos[b];
+  if (p < 0) {  // an idle sequence: nothing to see, nothing to store
+    if (split == 0) {
+      for (int i = threadIdx.x; i < heads * a.D; i += kThreads)
+        a.out[(static_cast<int64_t>(b) * a.Hk * a.G + h0) * a.D + i] = __float2bfloat16(0.f);
+      if (a.stored_k && chunk == 0)
+        for (int i = threadIdx.x; i < a.D; i += kThreads) {
+          a.stored_k[(static_cast<int64_t>(b) * a.Hk + hk) * a.D + i] = 0.f;
+          a.stored_v[(static_cast<int64_t>(b) * a.Hk + hk) * a.D + i] = 0.f;
+        }
+    }
+    return;
+  }
+  // the held rows, without the new token and without the row it replaces
+  const int held = static_cast<int>(p < a.slots ? p : a.slots);
+  const int fresh_slot = static_cast<int>(a.ring.slot(p));
+  int per = (held + a.splits - 1) / a.splits;
+  per = max((per + KT - 1) / KT * KT, kWarps * KT);
+  const int active = max(1, (held + per - 1) / per);
+  if (split >= active) return;
+  const int first = split * per, last = min(held, first + per);
+  const int tiles = (last - first + KT - 1) / KT;  // of this CTA; warp w takes w, w + 4, ...
+  const int64_t bh = static_cast<int64_t>(b) * a.Hk + hk;
+  const int64_t base = bh * a.ring.alloc;
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < kWarps * ST; ++i) mbar_init(&bars[i], 1);
+    fence_barrier_init();
+  }
+  __syncthreads();
+
+  uint8_t* ring = smem + warp * ST * C::kStage;
+  uint64_t* full = bars + warp * ST;
+  auto load = [&](int i) {  // tile i of this warp (one lane)
+    const int stage = i % ST;
+    const int64_t row = base + first + (warp + i * kWarps) * KT;
+    uint8_t* dst = ring + stage * C::kStage;
+    mbar_arrive_expect_tx(&full[stage], C::kStage);
+    if (BITS == 16) {
+#pragma unroll
+      for (int c = 0; c < DP / 64; ++c) {
+        tma_load_2d(dst + c * KT * 128, &tmK, &full[stage], c * 64, static_cast<int>(row));
+        tma_load_2d(dst + C::kOperand + c * KT * 128, &tmV, &full[stage], c * 64, static_cast<int>(row));
+      }
+    } else {
+      bulk_load(dst, a.ks.rows + row * C::kRowBytes, C::kOperand, &full[stage]);
+      bulk_load(dst + C::kOperand, a.vs.rows + row * C::kRowBytes, C::kOperand, &full[stage]);
+      bulk_load(dst + 2 * C::kOperand, a.ks.params + row * NG, KT * C::kParamBytes, &full[stage]);
+      bulk_load(dst + 2 * C::kOperand + KT * C::kParamBytes, a.vs.params + row * NG, KT * C::kParamBytes, &full[stage]);
+    }
+  };
+  const int mine = tiles > warp ? (tiles - warp + kWarps - 1) / kWarps : 0;
+  int loaded = 0;
+  if (lane == 0)
+    for (; loaded < min(mine, ST); ++loaded) load(loaded);
+  __syncwarp();
+
+  // Query rows as the A operand. Channels of k-step kk that thread t holds: for
+  // bf16 keys (kk/4)*64 + t*16 + (kk%4)*4 + 0..3, for packed keys (kk/2)*32 +
+  // t*8 + (kk%2)*4 + 0..3.
+  uint32_t qa[DP / 16][2];
+  float qsum[NG];
+  {
+    const __nv_bfloat16* qrow = a.q + b * a.q_b + (h0 + n) * a.q_h;
+#pragma unroll
+    for (int kk = 0; kk < DP / 16; ++kk) {
+      const int c = BITS == 16 ? (kk >> 2) * 64 + t * 16 + (kk & 3) * 4 : (kk >> 1) * 32 + t * 8 + (kk & 1) * 4;
+      const uint2 w = (n < heads && c < a.D) ? *reinterpret_cast<const uint2*>(qrow + c) : make_uint2(0u, 0u);
+      qa[kk][0] = w.x;
+      qa[kk][1] = w.y;
+    }
+#pragma unroll
+    for (int g = 0; g < NG; ++g) {
+      float x = 0.f;
+      if (BITS == 4) {
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+#pragma unroll
+          for (int w = 0; w < 2; ++w)
+            x += __uint_as_float(qa[2 * g + e][w] << 16) + __uint_as_float(qa[2 * g + e][w] & 0xffff0000u);
+        x += __shfl_xor_sync(0xffffffff, x, 1);
+        x += __shfl_xor_sync(0xffffffff, x, 2);
+      }
+      qsum[g] = x;
+    }
+  }
+
+  State<DP, BITS> st;
+  st.m = -INFINITY;
+  st.l = 0.f;
+#pragma unroll
+  for (int i = 0; i < DP / 8; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) st.o[i][j] = 0.f;
+  if (BITS == 4) {
+#pragma unroll
+    for (int g = 0; g < NG; ++g) st.c[g] = 0.f;
+  }
+
+  // The new token: its row into the cache (once) and, laid out as a tile of one
+  // key, into this warp's result.
+  if (split == 0 && warp == 0) {
+    constexpr int L = DP / 8;
+    const bool value = lane >= L;
+    const int i = lane % L;
+    const View& x = value ? a.v : a.k;
+    const Store& s = value ? a.vs : a.ks;
+    const bool on = lane < 2 * L;
+    const uint4 u = on ? load8(x.p + b * x.b + hk * x.h, i, a.D) : make_uint4(0, 0, 0, 0);
+    const int64_t row = base + fresh_slot;
+    uint8_t* tile = fresh + (value ? 16 * C::kRowBytes : 0);
+    uint32_t* params = reinterpret_cast<uint32_t*>(fresh + 32 * C::kRowBytes) + (value ? 16 * NG : 0);
+    float f[8];
+    unpack8(u, f);
+    if (BITS == 16) {
+      if (on) {
+        *reinterpret_cast<uint4*>(tile + (i >> 3) * 16 * 128 + ((i & 7) << 4)) = u;  // row 0: chunks in order
+        if (chunk == 0) *reinterpret_cast<uint4*>(s.rows + row * C::kRowBytes + i * 16) = u;
+      }
+    } else {
+      const Quant8 q = quantize8(f);
+      values8(q, f);
+      if (on) {
+        uint8_t* dst = s.rows + row * C::kRowBytes;
+        if (value) {
+          put_value8<DP>(tile, i, q.code);
+          if (chunk == 0) put_value8<DP>(dst, i, q.code);
+        } else {
+          put_key8<DP>(tile, i, q.code);
+          if (chunk == 0) put_key8<DP>(dst, i, q.code);
+        }
+        if ((i & 3) == 0) {
+          params[i >> 2] = q.param;
+          if (chunk == 0) s.params[row * NG + (i >> 2)] = q.param;
+        }
+      }
+    }
+    if (a.stored_k && chunk == 0 && on && i * 8 < a.D)
+      store8f((value ? a.stored_v : a.stored_k) + bh * a.D + i * 8, f);
+    __syncwarp();
+    const uint32_t* fp = reinterpret_cast<const uint32_t*>(fresh + 32 * C::kRowBytes);
+    attend<DP, BITS, 1>(st, qa, qsum, fresh, fresh + 16 * C::kRowBytes, fp, fp + 16 * NG, 16, 1u, a.scale_log2);
+  }
+
+  bool ok = true;
+  for (int i = 0; i < mine && ok; ++i) {
+    const int stage = i % ST;
+    ok = __all_sync(0xffffffff, mbar_wait(&full[stage], (i / ST) & 1, a.status, kTimeoutTmaFull));
+    if (!ok) break;
+    const uint8_t* src = ring + stage * C::kStage;
+    const uint32_t* pk = reinterpret_cast<const uint32_t*>(src + 2 * C::kOperand);
+    const uint32_t* pv = pk + KT * NG;
+    const int row = first + (warp + i * kWarps) * KT;
+    constexpr int NS = KT % 32 == 0 ? 2 : 1;
+#pragma unroll 1
+    for (int u = 0; u < KT / (16 * NS); ++u) {
+      const int r = row + u * 16 * NS;
+      if (r >= last) break;
+      constexpr uint32_t kAll = NS == 2 ? 0xffffffffu : 0xffffu;
+      uint32_t valid = last - r >= 16 * NS ? kAll : (1u << (last - r)) - 1u;
+      if (fresh_slot >= r && fresh_slot < r + 16 * NS) valid &= ~(1u << (fresh_slot - r));
+      const int off = u * 16 * NS;
+      attend<DP, BITS, NS>(st, qa, qsum, src + off * (BITS == 16 ? 128 : C::kRowBytes),
+                           src + C::kOperand + off * (BITS == 16 ? 128 : C::kRowBytes), pk + off * NG, pv + off * NG,
+                           KT, valid, a.scale_log2);
+    }
+    __syncwarp();
+    if (lane == 0 && loaded < mine) load(loaded++);
+    __syncwarp();
+  }
+  if (!ok && lane == 0)  // a wait expired: no copy may land after the CTA is gone
+    for (int i = max(0, loaded - ST); i < loaded; ++i) mbar_wait(&full[i % ST], (i / ST) & 1, a.status, kTimeoutTmaFull);
+
+  // the keys of a row were spread over 4 lanes
+  st.l += __shfl_xor_sync(0xffffffff, st.l, 1);
+  st.l += __shfl_xor_sync(0xffffffff, st.l, 2);
+  if (BITS == 4) {
+#pragma unroll
+    for (int g = 0; g < NG; ++g) {
+      st.c[g] += __shfl_xor_sync(0xffffffff, st.c[g], 1);
+      st.c[g] += __shfl_xor_sync(0xffffffff, st.c[g], 2);
+    }
+  }
+  __syncthreads();  // every ring has been read
+  float* join = reinterpret_cast<float*>(smem);  // [warp][row][DP + 2]: output, m, l
+  if (n < heads) {
+    float* row = join + (warp * kRows + n) * (DP + 2);
+#pragma unroll
+    for (int i = 0; i < DP / 8; ++i) {
+      const float c = BITS == 4 ? st.c[i >> 2] : 0.f;
+      row[channel_of<DP, BITS>(i, 2 * t)] = st.o[i][0] + st.o[i][2] + c;
+      row[channel_of<DP, BITS>(i, 2 * t + 1)] = st.o[i][1] + st.o[i][3] + c;
+    }
+    if (t == 0) {
+      row[DP] = st.m;
+      row[DP + 1] = st.l;
+    }
+  }
+  __syncthreads();
+  const int64_t unit = bh * a.chunks + chunk;
+  float* part = a.partial + (unit * a.splits + split) * (kRows * (DP + 2));
+  for (int i = threadIdx.x; i < heads * DP; i += kThreads) {
+    const int r = i / DP, d = i % DP;
+    float m = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) m = fmaxf(m, join[(w * kRows + r) * (DP + 2) + DP]);
+    const float m_use = m == -INFINITY ? 0.f : m;
+    float o = 0.f, l = 0.f;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+      const float* row = join + (w * kRows + r) * (DP + 2);
+      const float c = exp2f(row[DP] - m_use);
+      o += c * row[d];
+      l += c * row[DP + 1];
+    }
+    if (active == 1) {
+      if (d < a.D) a.out[(static_cast<int64_t>(b) * a.Hk * a.G + h0 + r) * a.D + d] = __float2bfloat16(o / l);
+    } else {
+      part[r * (DP + 2) + d] = o;
+      if (d == 0) {
+        part[r * (DP + 2) + DP] = m;
+        part[r * (DP + 2) + DP + 1] = l;
+      }
+    }
+  }
+  if (active == 1) return;
+  __threadfence();
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    const int before = atomicAdd(&a.arrived[unit], 1);
+    *last_flag = before == active - 1;
+    if (before == active - 1) a.arrived[unit] = 0;  // ready for the next launch
+  }
+  __syncthreads();
+  if (!*last_flag) return;
+  __threadfence();
+  const float* all = a.partial + unit * a.splits * (kRows * (DP + 2));
+  for (int i = threadIdx.x; i < heads * DP; i += kThreads) {
+    const int r = i / DP, d = i % DP;
+    const float* row = all + r * (DP + 2);
+    constexpr int64_t kStep = kRows * (DP + 2);
+    float m = -INFINITY;
+    for (int s = 0; s < active; ++s) m = fmaxf(m, __ldcg(row + s * kStep + DP));
+    float o = 0.f, l = 0.f;
+#pragma unroll 4
+    for (int s = 0; s < active; ++s) {
+      const float c = exp2f(__ldcg(row + s * kStep + DP) - m);
+      o += c * __ldcg(row + s * kStep + d);
+      l += c * __ldcg(row + s * kStep + DP + 1);
+    }
+    if (d < a.D) a.out[(static_cast<int64_t>(b) * a.Hk * a.G + h0 + r) * a.D + d] = __float2bfloat16(o / l);
+  }
+}
+
+// -------------------------------------------------------------------- host
+int padded_dim(int64_t D) { return D <= 64 ? 64 : 128; }
+
+struct Cache {  // the tensors of one cache, checked
+  int64_t B, Hk, alloc, D;
+  int DP, bits;
+  Store ks, vs;
+};
+
+Cache check_cache(const at::Tensor& keys, const at::Tensor& values, const c10::optional<at::Tensor>& key_params,
+                  const c10::optional<at::Tensor>& value_params, int64_t D, int64_t slots) {
+  Cache c;
+  TORCH_CHECK(D >= 8 && D <= 128 && D % 8 == 0, "kv cache: head_dim must be a multiple of 8 up to 128, got ",
+              std::to_string(D));
+  c.D = D;
+  c.DP = padded_dim(D);
+  c.bits = keys.scalar_type() == at::kBFloat16 ? 16 : 4;
+  TORCH_CHECK(c.bits == 16 || (keys.scalar_type() == at::kByte && D % 32 == 0),
+              "kv cache: bf16 rows, or uint8 rows with head_dim a multiple of 32");
+  const int64_t row = c.bits == 16 ? c.DP : c.DP / 2;
+  for (const at::Tensor* x : {&keys, &values})
+    TORCH_CHECK(x->is_cuda() && x->is_contiguous() && x->dim() == 4 && x->size(3) == row &&
+                    x->scalar_type() == keys.scalar_type() && x->sizes() == keys.sizes() &&
+                    x->device() == keys.device() && reinterpret_cast<uintptr_t>(x->data_ptr()) % 16 == 0,
+                "kv cache: contiguous, aligned keys and values [B, Hk, slots, ", std::to_string(row), "] required");
+  c.B = keys.size(0);
+  c.Hk = keys.size(1);
+  c.alloc = keys.size(2);
+  TORCH_CHECK(c.alloc % 64 == 0 && slots >= 1 && slots <= c.alloc, "kv cache: slots in whole tiles of 64 required");
+  TORCH_CHECK(c.B >= 1 && c.B <= 65535 && c.Hk >= 1 && c.Hk <= 32767, "kv cache: batch or heads out of range");
+  TORCH_CHECK(c.B * c.Hk * c.alloc < (int64_t(1) << 31), "kv cache: more than 2^31 rows");
+  c.ks = {static_cast<uint8_t*>(keys.data_ptr()), nullptr};
+  c.vs = {static_cast<uint8_t*>(values.data_ptr()), nullptr};
+  if (c.bits == 4) {
+    TORCH_CHECK(key_params.has_value() && value_params.has_value(), "kv cache: 4-bit rows need their parameters");
+    for (const at::Tensor* x : {&*key_params, &*value_params})
+      TORCH_CHECK(x->is_cuda() && x->is_contiguous() && x->scalar_type() == at::kInt && x->dim() == 4 &&
+                      x->size(0) == c.B && x->size(1) == c.Hk && x->size(2) == c.alloc && x->size(3) == c.DP / 32 &&
+                      x->device() == keys.device() && reinterpret_cast<uintptr_t>(x->data_ptr()) % 16 == 0,
+                  "kv cache: contiguous int32 parameters [B, Hk, slots, ", std::to_string(c.DP / 32), "] required");
+    c.ks.params = reinterpret_cast<uint32_t*>(key_params->data_ptr());
+    c.vs.params = reinterpret_cast<uint32_t*>(value_params->data_ptr());
+  }
+  return c;
+}
+
+Ring ring_of(const Cache& c, int64_t window, int64_t sinks, int64_t slots) {
+  TORCH_CHECK(window >= 1 && sinks >= 0 && window + sinks == slots, "kv cache: window + sinks must be the slots");
+  return {window, sinks, static_cast<int>(c.alloc)};
+}
+
+void check_rows(const at::Tensor& x, const Cache& c, const at::Tensor& keys, const char* name) {
+  TORCH_CHECK(x.is_cuda() && x.device() == keys.device() && x.scalar_type() == at::kBFloat16 && x.stride(-1) == 1 &&
+                  reinterpret_cast<uintptr_t>(x.data_ptr()) % 16 == 0 && x.size(0) == c.B && x.size(-1) == c.D,
+              "kv cache: ", name, " must be CUDA bf16 with unit inner stride, 16-byte aligned, of the cache's batch "
+              "and head_dim");
+  for (int i = 0; i + 1 < x.dim(); ++i)
+    TORCH_CHECK(x.size(i) == 1 || x.stride(i) % 8 == 0, "kv cache: ", name, " strides must be multiples of 8 elements");
+}
+
+void check_positions(const at::Tensor& x, const Cache& c, const at::Tensor& keys, const char* name) {
+  TORCH_CHECK(x.is_cuda() && x.device() == keys.device() && x.scalar_type() == at::kLong && x.is_contiguous() &&
+                  x.dim() == 1 && x.size(0) == c.B,
+              "kv cache: ", name, " must be a contiguous CUDA int64 tensor [B]");
+}
+
+template <typename F>
+void dispatch(const Cache& c, F&& f) {
+  if (c.DP == 64) {
+    if (c.bits == 16)
+      f(std::integral_constant<int, 64>(), std::integral_constant<int, 16>());
+    else
+      f(std::integral_constant<int, 64>(), std::integral_constant<int, 4>());
+  } else {
+    if (c.bits == 16)
+      f(std::integral_constant<int, 128>(), std::integral_constant<int, 16>());
+    else
+      f(std::integral_constant<int, 128>(), std::integral_constant<int, 4>());
+  }
+}
+
+}  // namespace kv_cache
+}  // namespace dst
+
+using namespace dst;
+
+using OptTensor = c10::optional<at::Tensor>;
+
+// k, v [B, T, Hk, D]: the visible tokens of each prompt into the cache; pos[b] = its length.
+void kv_cache_fill(const at::Tensor& k, const at::Tensor& v, const OptTensor& lengths, const at::Tensor& pos,
+                   const at::Tensor& keys, const at::Tensor& values, const OptTensor& key_params,
+                   const OptTensor& value_params, int64_t window, int64_t sinks) {
+  using namespace kv_cache;
+  const int64_t slots = window + sinks;
+  TORCH_CHECK(k.dim() == 4 && v.dim() == 4 && k.sizes() == v.sizes(), "kv cache: k and v [B, T, Hk, D] required");
+  const Cache c = check_cache(keys, values, key_params, value_params, k.size(3), slots);
+  const Ring ring = ring_of(c, window, sinks, slots);
+  check_rows(k, c, keys, "k");
+  check_rows(v, c, keys, "v");
+  TORCH_CHECK(k.size(2) == c.Hk, "kv cache: k and v must have the cache's heads");
+  TORCH_CHECK(k.size(1) >= 1 && k.size(1) < (int64_t(1) << 31), "kv cache: prompt length out of range");
+  if (lengths) check_positions(*lengths, c, keys, "lengths");
+  check_positions(pos, c, keys, "pos");
+  c10::cuda::CUDAGuard guard(keys.device());
+  const int T = static_cast<int>(k.size(1));
+  const int rows = static_cast<int>(std::min<int64_t>(T, slots));
+  const View kv = {static_cast<const __nv_bfloat16*>(k.data_ptr()), k.stride(0), k.stride(2), k.stride(1)};
+  const View vv = {static_cast<const __nv_bfloat16*>(v.data_ptr()), v.stride(0), v.stride(2), v.stride(1)};
+  dispatch(c, [&](auto dp, auto bits) {
+    const int64_t threads = static_cast<int64_t>(rows) * (dp() / 8);
+    const dim3 grid(static_cast<unsigned>((threads + 255) / 256), static_cast<unsigned>(2 * c.Hk), static_cast<unsigned>(c.B));
+    fill_kernel<dp(), bits()><<<grid, 256, 0, at::cuda::getCurrentCUDAStream()>>>(
+        kv, vv, lengths ? lengths->data_ptr<int64_t>() : nullptr, pos.data_ptr<int64_t>(), c.ks, c.vs, ring, T, rows,
+        static_cast<int>(c.Hk), static_cast<int>(c.D), status_ptr());
+  });
+  C10_CUDA_KERNEL_LAUNCH_CHECK();
+}
+
+// The held rows [B, Hk, slots, D] in slot order: bf16, or fp32 for 4 bits.
+std::vector<at::Tensor> kv_cache_read(const at::Tensor& pos, const at::Tensor& keys, const at::Tensor& values,
+                                      const OptTensor& key_params, const OptTensor& value_params, int64_t window,
+                                      int64_t sinks, int64_t D) {
+  using namespace kv_cache;
+  const int64_t slots = window + sinks;
+  const Cache c = check_cache(keys, values, key_params, value_params, D, slots);
+  const Ring ring = ring_of(c, window, sinks, slots);
+  check_positions(pos, c, keys, "pos");
+  c10::cuda::CUDAGuard guard(keys.device());
+  auto options = keys.options().dtype(c.bits == 16 ? at::kBFloat16 : at::kFloat);
+  at::Tensor ko = at::empty({c.B, c.Hk, slots, D}, options), vo = at::empty({c.B, c.Hk, slots, D}, options);
+  dispatch(c, [&](auto dp, auto bits) {
+    const int64_t threads = slots * (dp() / 8);
+    const dim3 grid(static_cast<unsigned>((threads + 255) / 256), static_cast<unsigned>(2 * c.Hk), static_cast<unsigned>(c.B));
+    read_kernel<dp(), bits()><<<grid, 256, 0, at::cuda::getCurrentCUDAStream()>>>(
+        c.ks, c.vs, pos.data_ptr<int64_t>(), ko.data_ptr(), vo.data_ptr(), ring, static_cast<int>(slots),
+        static_cast<int>(c.Hk), static_cast<int>(D));
+  });
+  C10_CUDA_KERNEL_LAUNCH_CHECK();
+  return {ko, vo};
+}
+
+// How many CTAs share the slots of one (sequence, key head), and the floats and
+// counters that joining them takes: enough CTAs to fill the GPU, each with at
+// least one tile per warp.
+std::vector<int64_t> kv_cache_plan(int64_t batch, int64_t kv_heads, int64_t heads, int64_t D, int64_t slots, bool packed) {
+  using namespace kv_cache;
+  TORCH_CHECK(batch >= 1 && kv_heads >= 1 && heads >= 1 && heads % kv_heads == 0 && slots >= 1,
+              "kv cache: query heads must be a multiple of the key heads");
+  const int64_t chunks = (heads / kv_heads + kRows - 1) / kRows, units = batch * kv_heads * chunks;
+  const int DP = padded_dim(D);
+  const int64_t tile = packed ? (DP == 64 ? 64 : 32) : (DP == 64 ? 32 : 16);
+  const int64_t ctas = packed ? (DP == 64 ? 4 : 3) : 2;
+  const int64_t most = std::max<int64_t>(1, (slots + kWarps * tile - 1) / (kWarps * tile));
+  const int64_t splits = std::min(most, std::max<int64_t>(1, (ctas * num_sms() + units - 1) / units));
+  return {splits, units * splits * kRows * (DP + 2), units};
+}
+
+// One token per sequence: q [B, H, D], k and v [B, Hk, D], pos [B] (-1: idle).
+// Returns the attention [B, H, D] over the cache with the token in it, and (on
+// request) what the stored rows stand for, fp32 [B, Hk, D].
+std::vector<at::Tensor> kv_cache_step(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
+                                      const at::Tensor& pos, const at::Tensor& keys, const at::Tensor& values,
+                                      const OptTensor& key_params, const OptTensor& value_params,
+                                      const at::Tensor& partial, const at::Tensor& arrived, int64_t window,
+                                      int64_t sinks, int64_t splits, bool return_stored) {
+  using namespace kv_cache;
+  const int64_t slots = window + sinks;
+  TORCH_CHECK(q.dim() == 3 && k.dim() == 3 && v.dim() == 3 && k.sizes() == v.sizes(),
+              "kv cache: q [B, H, D] and k, v [B, Hk, D] required");
+  const Cache c = check_cache(keys, values, key_params, value_params, q.size(2), slots);
+  const Ring ring = ring_of(c, window, sinks, slots);
+  check_rows(q, c, keys, "q");
+  check_rows(k, c, keys, "k");
+  check_rows(v, c, keys, "v");
+  check_positions(pos, c, keys, "pos");
+  TORCH_CHECK(k.size(1) == c.Hk && q.size(1) >= 1 && q.size(1) % c.Hk == 0,
+              "kv cache: query heads must be a multiple of the cache's heads");
+  const int64_t H = q.size(1), G = H / c.Hk, chunks = (G + kRows - 1) / kRows, units = c.B * c.Hk * chunks;
+  TORCH_CHECK(c.Hk * chunks <= 65535, "kv cache: too many heads");
+  TORCH_CHECK(splits >= 1 && splits <= 65535 && partial.is_cuda() && partial.device() == keys.device() &&
+                  partial.is_contiguous() && partial.scalar_type() == at::kFloat &&
+                  partial.numel() >= units * splits * kRows * (c.DP + 2) && arrived.is_cuda() &&
+                  arrived.device() == keys.device() && arrived.is_contiguous() &&
+                  arrived.scalar_type() == at::kInt && arrived.numel() >= units,
+              "kv cache: workspace too small for this call");
+  c10::cuda::CUDAGuard guard(keys.device());
+  at::Tensor out = at::empty({c.B, H, c.D}, q.options());
+  std::vector<at::Tensor> result = {out};
+  StepArgs a;
+  a.q = static_cast<const __nv_bfloat16*>(q.data_ptr());
+  a.q_b = q.stride(0), a.q_h = q.stride(1);
+  a.k = {static_cast<const __nv_bfloat16*>(k.data_ptr()), k.stride(0), k.stride(1), 0};
+  a.v = {static_cast<const __nv_bfloat16*>(v.data_ptr()), v.stride(0), v.stride(1), 0};
+  a.pos = pos.data_ptr<int64_t>();
+  a.ks = c.ks, a.vs = c.vs;
+  a.out = static_cast<__nv_bfloat16*>(out.data_ptr());
+  a.stored_k = a.stored_v = nullptr;
+  if (return_stored) {
+    for (int i = 0; i < 2; ++i) result.push_back(at::empty({c.B, c.Hk, c.D}, q.options().dtype(at::kFloat)));
+    a.stored_k = result[1].data_ptr<float>();
+    a.stored_v = result[2].data_ptr<float>();
+  }
+  a.partial = partial.data_ptr<float>();
+  a.arrived = arrived.data_ptr<int>();
+  a.ring = ring;
+  a.slots = static_cast<int>(slots), a.Hk = static_cast<int>(c.Hk), a.G = static_cast<int>(G);
+  a.D = static_cast<int>(c.D), a.chunks = static_cast<int>(chunks), a.splits = static_cast<int>(splits);
+  a.scale_log2 = static_cast<float>(1.4426950408889634 / std::sqrt(static_cast<double>(c.D)));
+  a.status = status_ptr();
+  const dim3 grid(static_cast<unsigned>(splits), static_cast<unsigned>(c.Hk * chunks), static_cast<unsigned>(c.B));
+  dispatch(c, [&](auto dp, auto bits) {
+    using C = StepCfg<dp(), bits()>;
+    CUtensorMap tk{}, tv{};
+    if (bits() == 16) {
+      const uint64_t rows = static_cast<uint64_t>(c.B) * c.Hk * c.alloc;
+      tk = make_tmap_bf16(keys.data_ptr(), dp(), rows, dp(), 64, C::KT);
+      tv = make_tmap_bf16(values.data_ptr(), dp(), rows, dp(), 64, C::KT);
+    }
+    auto kernel = step_kernel<dp(), bits()>;
+    C10_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem));
+    kernel<<<grid, kThreads, C::kSmem, at::cuda::getCurrentCUDAStream()>>>(tk, tv, a);
+  });
+  C10_CUDA_KERNEL_LAUNCH_CHECK();
+  return result;
+}
+
+void register_kv_cache(pybind11::module& m) {
+  namespace py = pybind11;
+  m.def("kv_cache_fill", &kv_cache_fill, "prompt rows into a rolling key/value cache", py::arg("k"), py::arg("v"),
+        py::arg("lengths"), py::arg("pos"), py::arg("keys"), py::arg("values"), py::arg("key_params"),
+        py::arg("value_params"), py::arg("window"), py::arg("sinks"));
+  m.def("kv_cache_read", &kv_cache_read, "held rows of a rolling key/value cache", py::arg("pos"), py::arg("keys"),
+        py::arg("values"), py::arg("key_params"), py::arg("value_params"), py::arg("window"), py::arg("sinks"),
+        py::arg("D"));
+  m.def("kv_cache_plan", &kv_cache_plan, "splits, partial floats and counters of a step", py::arg("batch"),
+        py::arg("kv_heads"), py::arg("heads"), py::arg("D"), py::arg("slots"), py::arg("packed"));
+  m.def("kv_cache_step", &kv_cache_step, "one token per sequence over a rolling key/value cache", py::arg("q"),
+        py::arg("k"), py::arg("v"), py::arg("pos"), py::arg("keys"), py::arg("values"), py::arg("key_params"),
+        py::arg("value_params"), py::arg("partial"), py::arg("arrived"), py::arg("window"), py::arg("sinks"),
+        py::arg("splits"), py::arg("return_stored"));
+}

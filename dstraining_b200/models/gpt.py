@@ -74,8 +74,16 @@ class GPTConfig:
     # Full activation recompute (not in the reference): each block keeps only
     # its input and re-runs its forward in backward.
     recompute_blocks: bool = False
+    # Sliding-window attention (not in the reference): each token sees its last
+    # `attention_window` tokens (0: all) and the first `attention_sinks`.
+    attention_window: int = 0
+    attention_sinks: int = 0
 
     def __post_init__(self):
+        if self.attention_window < 0 or self.attention_sinks < 0:
+            raise ValueError("attention_window and attention_sinks must not be negative")
+        if self.attention_sinks and not self.attention_window:
+            raise ValueError("attention_sinks without attention_window: every token is visible already")
         if self.dropout != 0.0:
             # No RNG discipline across TP ranks / recompute is implemented, as
             # in the reference; refuse instead of training something else.
@@ -113,7 +121,8 @@ class CausalSelfAttention(nn.Module):
 
     def forward(self, x: torch.Tensor, residual: Optional[torch.Tensor] = None) -> torch.Tensor:
         qkv = self.qkv(x)  # sequence is full here even under SP
-        y = causal_attention(qkv, self.n_head_local, self.head_dim, self.config.recompute_attention)
+        y = causal_attention(qkv, self.n_head_local, self.head_dim, self.config.recompute_attention,
+                             self.config.attention_window, self.config.attention_sinks)
         return self.proj(y, residual=residual)
 
 

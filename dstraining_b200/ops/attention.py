@@ -12,6 +12,9 @@ rank whole heads. Output is ``[B, T, h * d]``.
   runs give bit-identical gradients.
 * otherwise: :func:`core_attention`, the materialised reference algorithm,
   optionally wrapped in :func:`recompute`.
+
+With a ``window`` the layer is sliding-window attention with sinks
+(:mod:`dstraining_b200.ops.window`) on both paths.
 """
 
 from __future__ import annotations
@@ -36,7 +39,15 @@ def core_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor) -> torch.T
     return probs @ v
 
 
-def causal_attention(qkv: torch.Tensor, n_head: int, head_dim: int, recompute_core: bool) -> torch.Tensor:
+def causal_attention(qkv: torch.Tensor, n_head: int, head_dim: int, recompute_core: bool, window: int = 0,
+                     sinks: int = 0) -> torch.Tensor:
+    """``window`` 0: every token sees all before it."""
+    if window:
+        from .window import window_attention
+
+        if recompute_core and not native.active(qkv):
+            return recompute(lambda x: window_attention(x, n_head, head_dim, window, sinks), qkv)
+        return window_attention(qkv, n_head, head_dim, window, sinks)
     b, t, _ = qkv.shape
     if native.active(qkv):
         from .flash import flash_attention

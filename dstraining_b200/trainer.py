@@ -60,6 +60,9 @@ def add_args(p: argparse.ArgumentParser) -> argparse.ArgumentParser:
     p.add_argument("--micro", type=int, default=1, help="micro batch size (pipelines; with --grad-accum also pp=1)")
     p.add_argument("--grad-accum", action="store_true",
                    help="without pipelining: split each batch into --micro-sized micro-batches and accumulate")
+    p.add_argument("--window", type=int, default=0,
+                   help="sliding-window attention: each token sees its last N tokens (0: all)")
+    p.add_argument("--sinks", type=int, default=0, help="with --window: first tokens that stay visible")
     p.add_argument("--steps", type=int, default=50)
     p.add_argument("--lr", type=float, default=3e-4)
     p.add_argument("--lr-schedule", choices=["constant", "cosine"], default="constant")
@@ -151,6 +154,8 @@ class Trainer:
             recompute_attention=args.recompute,
             vocab_parallel_loss=args.vp,
             recompute_blocks=getattr(args, "recompute_blocks", False),
+            attention_window=getattr(args, "window", 0),
+            attention_sinks=getattr(args, "sinks", 0),
         )
         cfg = self.config
         if args.chunks > 1:

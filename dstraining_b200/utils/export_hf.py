@@ -38,6 +38,8 @@ from ..parallel.topology import SINGLE
 
 def hf_config(model: GPT) -> Dict:
     cfg = model.config
+    if cfg.attention_window:
+        raise ValueError("the Hugging Face GPT-2 layout has no sliding-window attention")
     return {
         "architectures": ["GPT2LMHeadModel"],
         "model_type": "gpt2",

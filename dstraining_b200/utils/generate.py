@@ -6,7 +6,9 @@
 ``generate(model, idx, ...)`` extends ``idx`` [B, T] token by token.
 ``temperature == 0`` is greedy decoding; otherwise tokens are sampled,
 optionally from the ``top_k`` most probable and / or the nucleus of
-probability ``top_p``.
+probability ``top_p``. With ``device_sampling`` (or ``min_p``) the tokens are
+drawn on the model's device by :func:`~dstraining_b200.ops.sampling.sample_tokens`
+and nothing is copied to the host per token.
 
 * With ``use_cache=True`` (the default) the prompt is run once and every
   later token costs one row per layer: its key and value are appended to a
@@ -17,6 +19,10 @@ probability ``top_p``.
   ``block_size`` the window slides and every step re-runs the whole window,
   exactly as without a cache. Runs on the model's own parameters with
   PyTorch ops (fp32 on CPU, the model's dtype on CUDA).
+* A model with an attention window, or ``cache_bits`` 16 or 4, decodes through
+  :class:`~dstraining_b200.ops.kv_cache.WindowCache`: ``sinks + window`` slots
+  per layer (the whole block without a window) in bf16 or 4 bits, appended to and
+  attended over in one kernel per layer on CUDA bf16.
 * Otherwise every step runs the model's full-context forward pass on the
   last ``block_size`` tokens, right-padded to a multiple of ``pad_to`` (the
   native causal attention kernels' 128-row tiles, so the sequence-parallel
@@ -41,6 +47,9 @@ import torch.distributed as dist
 import torch.nn.functional as F
 
 from ..models.gpt import GPT, GPTConfig
+from ..ops.kv_cache import WindowCache
+from ..ops.sampling import gumbel_noise, sample_tokens
+from ..ops.window import window_attention
 from ..parallel.comm import all_gather_dim
 from ..parallel.topology import SINGLE
 
@@ -52,18 +61,46 @@ class KVCache:
     tensor parallelism each rank caches its own heads; the row-parallel
     outputs are summed over the group (bias added once, after the sum) and the
     vocabulary-sharded logits gathered, so every rank sees the same logits -
-    every rank of the group must make the same calls."""
+    every rank of the group must make the same calls.
 
-    def __init__(self, model: GPT, batch: int):
+    With ``bits`` (or a model that has an attention window) the rows live in one
+    rolling :class:`WindowCache` per layer instead, and attention runs over it."""
+
+    def __init__(self, model: GPT, batch: int, bits: Optional[int] = None):
         cfg = model.config
         self.model = model
         self.tp = model.tp
         p = model.wte.weight
         self.H, self.D = cfg.n_head // self.tp.world, cfg.n_embd // cfg.n_head
+        self.len = 0
+        self.window = min(cfg.attention_window or cfg.block_size, cfg.block_size)
+        self.layers = None
+        if bits is not None or cfg.attention_window:
+            self.pos = torch.zeros(batch, dtype=torch.int64, device=p.device)  # shared by the layers
+            self.layers = [WindowCache(batch, self.H, self.D, self.window, cfg.attention_sinks, bits=bits or 16,
+                                       device=p.device, dtype=p.dtype, pos=self.pos) for _ in range(cfg.n_layer)]
+            return
         shape = (batch, self.H, cfg.block_size, self.D)
         self.k = [torch.empty(shape, dtype=p.dtype, device=p.device) for _ in range(cfg.n_layer)]
         self.v = [torch.empty(shape, dtype=p.dtype, device=p.device) for _ in range(cfg.n_layer)]
-        self.len = 0
+
+    def _attend(self, i: int, qkv: torch.Tensor, p0: int) -> torch.Tensor:
+        """Layer i's attention of qkv [B, t, H, 3, D] at positions p0.., its
+        keys and values appended -> [B, t, H * D]."""
+        b, t = qkv.shape[:2]
+        if self.layers is not None:
+            q, k, v = qkv.unbind(dim=3)
+            if p0 == 0:
+                self.layers[i].fill(k, v)
+                return window_attention(qkv.reshape(b, t, -1), self.H, self.D, self.window, self.layers[i].sinks)
+            return self.layers[i].step(q[:, 0], k[:, 0], v[:, 0], self.pos).reshape(b, t, -1)
+        q, k, v = (qkv[:, :, :, j].transpose(1, 2) for j in range(3))
+        self.k[i][:, :, p0 : p0 + t] = k
+        self.v[i][:, :, p0 : p0 + t] = v
+        keys, vals = self.k[i][:, :, : p0 + t], self.v[i][:, :, : p0 + t]
+        # the window's first pass is causal; a single new token sees every cached one
+        y = F.scaled_dot_product_attention(q, keys, vals, is_causal=p0 == 0 and t > 1)
+        return y.transpose(1, 2).reshape(b, t, self.H * self.D)
 
     @staticmethod
     def _ln(ln, x):
@@ -90,17 +127,12 @@ class KVCache:
         for i, blk in enumerate(m.blocks):
             a = blk.attn
             qkv = F.linear(self._ln(blk.ln_1, x), a.qkv.weight, a.qkv.bias).view(b, t, self.H, 3, self.D)
-            q, k, v = (qkv[:, :, :, j].transpose(1, 2) for j in range(3))
-            self.k[i][:, :, p0 : p0 + t] = k
-            self.v[i][:, :, p0 : p0 + t] = v
-            keys, vals = self.k[i][:, :, : p0 + t], self.v[i][:, :, : p0 + t]
-            # the window's first pass is causal; a single new token sees every cached one
-            y = F.scaled_dot_product_attention(q, keys, vals, is_causal=p0 == 0 and t > 1)
-            y = y.transpose(1, 2).reshape(b, t, self.H * self.D)
-            x = x + self._row(y, a.proj)
+            x = x + self._row(self._attend(i, qkv, p0), a.proj)
             h = F.gelu(F.linear(self._ln(blk.ln_2, x), blk.mlp.c_fc.weight, blk.mlp.c_fc.bias), approximate="tanh")
             x = x + self._row(h, blk.mlp.c_proj)
         self.len = p0 + t
+        if self.layers is not None and p0:
+            self.pos += 1
         x = self._ln(m.ln_f, x[:, -1])
         logits = F.linear(x, m.lm_head.weight)  # this rank's vocabulary shard
         if self.tp.enabled:
@@ -142,9 +174,10 @@ def _full_context_logits(model: GPT, idx: torch.Tensor, pad_to: int) -> torch.Te
 @torch.no_grad()
 def generate(model: GPT, idx: torch.Tensor, max_new_tokens: int, temperature: float = 1.0,
              top_k: Optional[int] = None, generator: Optional[torch.Generator] = None, pad_to: int = 128,
-             use_cache: bool = True, top_p: Optional[float] = None) -> torch.Tensor:
+             use_cache: bool = True, top_p: Optional[float] = None, cache_bits: Optional[int] = None,
+             min_p: Optional[float] = None, device_sampling: bool = False) -> torch.Tensor:
     cfg = model.config
-    cache = KVCache(model, idx.shape[0]) if use_cache else None
+    cache = KVCache(model, idx.shape[0], cache_bits) if use_cache else None
     was_training = model.training
     model.eval()
     try:
@@ -155,7 +188,12 @@ def generate(model: GPT, idx: torch.Tensor, max_new_tokens: int, temperature: fl
                 logits = cache.forward(idx)
             else:
                 logits = cache.forward(idx[:, -1:])
-            nxt = _sample(logits, temperature, top_k, generator, top_p)
+            if device_sampling or min_p:
+                noise = gumbel_noise(*logits.shape, generator.device if generator is not None else logits.device, generator)
+                nxt = sample_tokens(logits, noise.to(logits.device), max(temperature, 0.0), top_k or 0,
+                                    1.0 if top_p is None else top_p, min_p or 0.0)[0][:, None]
+            else:
+                nxt = _sample(logits, temperature, top_k, generator, top_p)
             idx = torch.cat([idx, nxt.to(idx.dtype)], dim=1)
     finally:
         model.train(was_training)
@@ -189,6 +227,11 @@ def main(argv=None) -> None:
     ap.add_argument("--temperature", type=float, default=1.0)
     ap.add_argument("--top-k", type=int, default=None)
     ap.add_argument("--top-p", type=float, default=None, help="nucleus sampling")
+    ap.add_argument("--min-p", type=float, default=None,
+                    help="keep tokens at least this times as probable as the most probable (on the device)")
+    ap.add_argument("--cache-bits", type=int, choices=(16, 4), default=None,
+                    help="decode through the rolling key/value cache in bf16 or 4 bits")
+    ap.add_argument("--device-sampling", action="store_true", help="draw tokens on the model's device")
     ap.add_argument("--seed", type=int, default=0)
     ap.add_argument("--device", default="cuda" if torch.cuda.is_available() else "cpu")
     a = ap.parse_args(argv)
@@ -207,8 +250,10 @@ def main(argv=None) -> None:
         decode = (lambda out: bytes(t for t in out if t < 256).decode("utf-8", "replace")) if a.tokenizer == "bytes" \
             else (lambda out: tok.tok.decode(out))
     idx = torch.tensor([ids], dtype=torch.long, device=a.device)
-    g = torch.Generator().manual_seed(a.seed)
-    out = generate(model, idx, a.max_new_tokens, a.temperature, a.top_k, g, top_p=a.top_p)[0].tolist()
+    on_device = a.device_sampling or bool(a.min_p)
+    g = torch.Generator(device=a.device if on_device else "cpu").manual_seed(a.seed)
+    out = generate(model, idx, a.max_new_tokens, a.temperature, a.top_k, g, top_p=a.top_p, cache_bits=a.cache_bits,
+                   min_p=a.min_p, device_sampling=a.device_sampling)[0].tolist()
     print(decode(out) if decode else ",".join(map(str, out)))
 
 

@@ -76,9 +76,12 @@ def plan(args) -> Dict:
     head_dim = d // heads if heads else 0
     native = bool(getattr(args, "bf16", False))
     if native:
-        if head_dim not in (64, 128):
+        window = getattr(args, "window", 0)
+        if window and (head_dim % 8 or head_dim > 128):
+            warnings.append(f"head size {head_dim}: native window attention takes multiples of 8 up to 128")
+        if not window and head_dim not in (64, 128):
             warnings.append(f"head size {head_dim}: native attention takes 64 or 128")
-        if seq % 128:
+        if seq % 128 and not window:  # the window kernels run any length as it is
             warnings.append(f"sequence {seq} not a multiple of 128: attention zero-pads it to "
                             f"{-(-seq // 128) * 128} (padded rows computed and discarded)")
         if tp > 1:
