@@ -694,45 +694,61 @@ __global__ void __launch_bounds__(kThreads, DqCfg<DP>::kCtas)
 }
 
 // -------------------------------------------------------------------- host
-// [B, T, H, D] with unit inner stride; the other strides and the base must be
-// multiples of 16 bytes (a dimension of size 1 may have any stride).
-void check_operand(const at::Tensor& x, const char* name) {
-  TORCH_CHECK(x.dim() != 4 || (x.size(3) >= 8 && x.size(3) <= 128 && x.size(3) % 8 == 0),
-              "window attention: head_dim must be a multiple of 8 up to 128, got ",
-              std::to_string(x.size(3)));
-  TORCH_CHECK(x.is_cuda() && x.scalar_type() == at::kBFloat16 && x.dim() == 4, "window attention: ", name,
-              " must be a CUDA bf16 tensor [B, T, H, D]");
-  TORCH_CHECK(x.stride(3) == 1 && reinterpret_cast<uintptr_t>(x.data_ptr()) % 16 == 0, "window attention: ", name,
-              " needs a unit inner stride and a 16-byte aligned start");
+// Where q, k or v (or a gradient of one) lies: [B, T, heads, D] with unit inner
+// stride; the other strides and the start are multiples of 16 bytes, so that
+// tensor maps and 16-byte vectors can address it.
+struct Operand {
+  __nv_bfloat16* p;
+  Strides s;
+};
+
+bool addressable(const at::Tensor& x) {
+  if (x.stride(3) != 1 || reinterpret_cast<uintptr_t>(x.data_ptr()) % 16 != 0) return false;
   for (int i = 0; i < 3; ++i)
-    TORCH_CHECK(x.size(i) == 1 || (x.stride(i) > 0 && x.stride(i) % 8 == 0), "window attention: ", name,
-                " strides must be positive multiples of 8 elements");
+    if (x.size(i) != 1 && (x.stride(i) <= 0 || x.stride(i) % 8 != 0)) return false;
+  return true;
 }
 
-Strides strides_of(const at::Tensor& x) { return {x.stride(1), x.stride(2), x.stride(0)}; }
+at::Tensor as_addressable(const at::Tensor& x) {
+  return addressable(x) ? x : x.clone(at::MemoryFormat::Contiguous);
+}
 
-CUtensorMap map_of(const at::Tensor& x, int rows) {
-  const uint64_t dims[4] = {static_cast<uint64_t>(x.size(3)), static_cast<uint64_t>(x.size(1)),
-                            static_cast<uint64_t>(x.size(2)), static_cast<uint64_t>(x.size(0))};
-  const int axis[3] = {1, 2, 0};
+Operand operand(const at::Tensor& x) {
+  return {static_cast<__nv_bfloat16*>(x.data_ptr()), {x.stride(1), x.stride(2), x.stride(0)}};
+}
+
+// q, k or v of a buffer [B, T, heads, 3, D].
+Operand part_of(const at::Tensor& qkv, int which, int64_t D) {
+  return {static_cast<__nv_bfloat16*>(qkv.data_ptr()) + which * D, {qkv.stride(1), 3 * D, qkv.stride(0)}};
+}
+
+CUtensorMap map_of(const Operand& x, int64_t B, int64_t T, int64_t heads, int64_t D, int rows) {
+  const uint64_t dims[4] = {static_cast<uint64_t>(D), static_cast<uint64_t>(T), static_cast<uint64_t>(heads),
+                            static_cast<uint64_t>(B)};
+  const int64_t st[3] = {x.s.t, x.s.h, x.s.b};
   uint64_t strides[3];
-  for (int i = 0; i < 3; ++i) strides[i] = x.size(axis[i]) == 1 ? 16 : static_cast<uint64_t>(x.stride(axis[i])) * 2;
+  for (int i = 0; i < 3; ++i) strides[i] = dims[i + 1] == 1 ? 16 : static_cast<uint64_t>(st[i]) * 2;
   const uint32_t box[4] = {64, static_cast<uint32_t>(rows), 1, 1};
-  return make_tmap_bf16_4d(x.data_ptr(), dims, strides, box);
+  return make_tmap_bf16_4d(x.p, dims, strides, box);
 }
 
-Shape shape_of(const at::Tensor& q, const at::Tensor& k, int64_t window, int64_t sinks) {
-  const int64_t T = q.size(1), D = q.size(3);
-  TORCH_CHECK(T >= 1 && T < (int64_t(1) << 30) && q.size(0) >= 1, "window attention: T and B must be positive");
-  TORCH_CHECK(q.size(2) <= 65535 && q.size(0) <= 65535, "window attention: more than 65535 heads or sequences");
-  TORCH_CHECK(k.size(2) >= 1 && q.size(2) % k.size(2) == 0,
+void check_bf16(const at::Tensor& x, const char* name) {
+  TORCH_CHECK(x.is_cuda() && x.scalar_type() == at::kBFloat16, "window attention: ", name, " must be a CUDA bf16 tensor");
+}
+
+Shape shape_of(int64_t B, int64_t T, int64_t H, int64_t Hk, int64_t D, int64_t window, int64_t sinks) {
+  TORCH_CHECK(D >= 8 && D <= 128 && D % 8 == 0, "window attention: head_dim must be a multiple of 8 up to 128, got ",
+              std::to_string(D));
+  TORCH_CHECK(T >= 1 && T < (int64_t(1) << 30) && B >= 1, "window attention: T and B must be positive");
+  TORCH_CHECK(H <= 65535 && B <= 65535, "window attention: more than 65535 heads or sequences");
+  TORCH_CHECK(Hk >= 1 && H >= 1 && H % Hk == 0,
               "window attention: the number of query heads must be a multiple of the number of key heads");
   TORCH_CHECK(window >= 1 && sinks >= 0, "window attention: window >= 1 and sinks >= 0 required");
   Shape s;
   s.T = static_cast<int>(T);
   s.Tp = static_cast<int>((T + 127) / 128 * 128);
-  s.H = static_cast<int>(q.size(2));
-  s.G = static_cast<int>(q.size(2) / k.size(2));
+  s.H = static_cast<int>(H);
+  s.G = static_cast<int>(H / Hk);
   s.D = static_cast<int>(D);
   s.W = static_cast<int>(std::min(window, T));
   s.S = static_cast<int>(std::min(sinks, T));
@@ -743,107 +759,169 @@ Shape shape_of(const at::Tensor& q, const at::Tensor& k, int64_t window, int64_t
   return s;
 }
 
-template <typename K>
-void allow_smem(K kernel, int bytes) {
-  C10_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+template <auto kKernel>
+void allow_smem(int bytes) {  // once per kernel and device
+  static bool done[64] = {false};
+  int dev;
+  C10_CUDA_CHECK(cudaGetDevice(&dev));
+  if (!done[dev]) C10_CUDA_CHECK(cudaFuncSetAttribute(kKernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+  done[dev] = true;
 }
 
 template <int DP>
-void run_fwd(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const at::Tensor& out,
-             const at::Tensor& lse, const Shape& s) {
+void run_fwd(const Operand& q, const Operand& k, const Operand& v, __nv_bfloat16* out, float* lse, int64_t B,
+             const Shape& s) {
   constexpr int smem = FwdCfg<DP>::kSmem;
-  allow_smem(fwd_kernel<DP>, smem);
-  const dim3 grid(s.Tp / 128, s.H, static_cast<unsigned>(q.size(0)));
-  fwd_kernel<DP><<<grid, kThreads, smem, at::cuda::getCurrentCUDAStream()>>>(
-      map_of(q, 128), map_of(k, 64), map_of(v, 64), reinterpret_cast<__nv_bfloat16*>(out.data_ptr()),
-      lse.data_ptr<float>(), s);
+  allow_smem<fwd_kernel<DP>>(smem);
+  const int Hk = s.H / s.G;
+  fwd_kernel<DP><<<dim3(s.Tp / 128, s.H, static_cast<unsigned>(B)), kThreads, smem, at::cuda::getCurrentCUDAStream()>>>(
+      map_of(q, B, s.T, s.H, s.D, 128), map_of(k, B, s.T, Hk, s.D, 64), map_of(v, B, s.T, Hk, s.D, 64), out, lse, s);
   C10_CUDA_KERNEL_LAUNCH_CHECK();
 }
 
 template <int DP>
-void run_bwd(const at::Tensor& dout, const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
-             const at::Tensor& out, const at::Tensor& lse, const at::Tensor& di, const at::Tensor& dq,
-             const at::Tensor& dk, const at::Tensor& dv, const Shape& s) {
+void run_bwd(__nv_bfloat16* dout, const Operand& q, const Operand& k, const Operand& v, __nv_bfloat16* out,
+             const float* lse, float* di, const Operand& dq, const Operand& dk, const Operand& dv, int64_t B,
+             const Shape& s) {
   auto st = at::cuda::getCurrentCUDAStream();
-  auto bf = [](const at::Tensor& x) { return reinterpret_cast<__nv_bfloat16*>(x.data_ptr()); };
-  const float *l = lse.data_ptr<float>(), *d = di.data_ptr<float>();
-  const unsigned B = static_cast<unsigned>(q.size(0));
-  const int64_t rows = static_cast<int64_t>(B) * s.H * s.Tp;
+  const int Hk = s.H / s.G;
+  const int64_t rows = B * s.H * s.Tp;
   const int64_t blocks = (rows * (DP / 8) + 255) / 256;
   TORCH_CHECK(blocks < (int64_t(1) << 31), "window attention: too many rows");
-  rowdot_kernel<DP><<<static_cast<unsigned>(blocks), 256, 0, st>>>(bf(dout), bf(out), di.data_ptr<float>(), rows, s);
+  const Operand go = {dout, {static_cast<int64_t>(s.H) * s.D, s.D, static_cast<int64_t>(s.T) * s.H * s.D}};
+  rowdot_kernel<DP><<<static_cast<unsigned>(blocks), 256, 0, st>>>(dout, out, di, rows, s);
   C10_CUDA_KERNEL_LAUNCH_CHECK();
-  allow_smem(dkdv_kernel<DP>, DkdvCfg<DP>::kSmem);
-  dkdv_kernel<DP><<<dim3(s.Tp / 128, s.H / s.G, B), kThreads, DkdvCfg<DP>::kSmem, st>>>(
-      map_of(q, 64), map_of(dout, 64), map_of(k, 128), map_of(v, 128), l, d, bf(dk), bf(dv), strides_of(dk),
-      strides_of(dv), s);
+  allow_smem<dkdv_kernel<DP>>(DkdvCfg<DP>::kSmem);
+  dkdv_kernel<DP><<<dim3(s.Tp / 128, Hk, static_cast<unsigned>(B)), kThreads, DkdvCfg<DP>::kSmem, st>>>(
+      map_of(q, B, s.T, s.H, s.D, 64), map_of(go, B, s.T, s.H, s.D, 64), map_of(k, B, s.T, Hk, s.D, 128),
+      map_of(v, B, s.T, Hk, s.D, 128), lse, di, dk.p, dv.p, dk.s, dv.s, s);
   C10_CUDA_KERNEL_LAUNCH_CHECK();
-  allow_smem(dq_kernel<DP>, DqCfg<DP>::kSmem);
-  dq_kernel<DP><<<dim3(s.Tp / 128, s.H, B), kThreads, DqCfg<DP>::kSmem, st>>>(
-      map_of(q, 128), map_of(dout, 128), map_of(k, 64), map_of(v, 64), l, d, bf(dq), strides_of(dq), s);
+  allow_smem<dq_kernel<DP>>(DqCfg<DP>::kSmem);
+  dq_kernel<DP><<<dim3(s.Tp / 128, s.H, static_cast<unsigned>(B)), kThreads, DqCfg<DP>::kSmem, st>>>(
+      map_of(q, B, s.T, s.H, s.D, 128), map_of(go, B, s.T, s.H, s.D, 128), map_of(k, B, s.T, Hk, s.D, 64),
+      map_of(v, B, s.T, Hk, s.D, 64), lse, di, dq.p, dq.s, s);
   C10_CUDA_KERNEL_LAUNCH_CHECK();
 }
+
+// out [B, T, H, D] and the base-2 log-sum-exp [B, H, T rounded up to 128].
+std::pair<at::Tensor, at::Tensor> forward(const Operand& q, const Operand& k, const Operand& v, int64_t B,
+                                          const Shape& s, const at::TensorOptions& options) {
+  at::Tensor out = at::empty({B, s.T, s.H, s.D}, options);
+  at::Tensor lse = at::empty({B, s.H, s.Tp}, options.dtype(at::kFloat));
+  auto* o = static_cast<__nv_bfloat16*>(out.data_ptr());
+  if (s.D <= 64)
+    run_fwd<64>(q, k, v, o, lse.data_ptr<float>(), B, s);
+  else
+    run_fwd<128>(q, k, v, o, lse.data_ptr<float>(), B, s);
+  return {out, lse};
+}
+
+void backward(const at::Tensor& dout, const Operand& q, const Operand& k, const Operand& v, const at::Tensor& out,
+              const at::Tensor& lse, const Operand& dq, const Operand& dk, const Operand& dv, int64_t B, const Shape& s) {
+  at::Tensor go = dout.contiguous();
+  if (reinterpret_cast<uintptr_t>(go.data_ptr()) % 16) go = go.clone();
+  at::Tensor di = at::empty_like(lse);
+  auto *g = static_cast<__nv_bfloat16*>(go.data_ptr()), *o = static_cast<__nv_bfloat16*>(out.data_ptr());
+  if (s.D <= 64)
+    run_bwd<64>(g, q, k, v, o, lse.data_ptr<float>(), di.data_ptr<float>(), dq, dk, dv, B, s);
+  else
+    run_bwd<128>(g, q, k, v, o, lse.data_ptr<float>(), di.data_ptr<float>(), dq, dk, dv, B, s);
+}
+
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+
+// Separate q, k, v. The autograd nodes are C++: a Python node costs more host
+// time per call than a short sequence takes on the GPU.
+struct SeparateFn : public torch::autograd::Function<SeparateFn> {
+  static at::Tensor forward(AutogradContext* ctx, const at::Tensor& q_, const at::Tensor& k_, const at::Tensor& v_,
+                            int64_t window, int64_t sinks) {
+    c10::cuda::CUDAGuard guard(q_.device());
+    const int64_t B = q_.size(0), T = q_.size(1), D = q_.size(3);
+    const Shape s = shape_of(B, T, q_.size(2), k_.size(2), D, window, sinks);
+    const at::Tensor q = as_addressable(q_), k = as_addressable(k_), v = as_addressable(v_);
+    auto [out, lse] = attn_window::forward(operand(q), operand(k), operand(v), B, s, q.options());
+    ctx->save_for_backward({q, k, v, out, lse});
+    ctx->saved_data["window"] = window;
+    ctx->saved_data["sinks"] = sinks;
+    return out;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const auto saved = ctx->get_saved_variables();
+    const at::Tensor &q = saved[0], &k = saved[1], &v = saved[2], &out = saved[3], &lse = saved[4];
+    c10::cuda::CUDAGuard guard(q.device());
+    const Shape s = shape_of(q.size(0), q.size(1), q.size(2), k.size(2), q.size(3), ctx->saved_data["window"].toInt(),
+                             ctx->saved_data["sinks"].toInt());
+    at::Tensor dq = at::empty(q.sizes(), q.options()), dk = at::empty(k.sizes(), k.options()),
+               dv = at::empty(v.sizes(), v.options());
+    attn_window::backward(grads[0], operand(q), operand(k), operand(v), out, lse, operand(dq), operand(dk), operand(dv),
+                          q.size(0), s);
+    debug_check("window_attention backward");
+    return {dq, dk, dv, at::Tensor(), at::Tensor()};
+  }
+};
+
+// q, k, v interleaved head by head in one buffer, and their gradients likewise.
+struct FusedFn : public torch::autograd::Function<FusedFn> {
+  static at::Tensor forward(AutogradContext* ctx, const at::Tensor& qkv_, int64_t n_head, int64_t head_dim,
+                            int64_t window, int64_t sinks) {
+    c10::cuda::CUDAGuard guard(qkv_.device());
+    const int64_t B = qkv_.size(0), T = qkv_.size(1);
+    const Shape s = shape_of(B, T, n_head, n_head, head_dim, window, sinks);
+    at::Tensor qkv = qkv_.contiguous();
+    if (reinterpret_cast<uintptr_t>(qkv.data_ptr()) % 16) qkv = qkv.clone();
+    auto [out, lse] = attn_window::forward(part_of(qkv, 0, head_dim), part_of(qkv, 1, head_dim),
+                                           part_of(qkv, 2, head_dim), B, s, qkv.options());
+    ctx->save_for_backward({qkv, out, lse});
+    ctx->saved_data["window"] = window;
+    ctx->saved_data["sinks"] = sinks;
+    return out.view({B, T, n_head * head_dim});
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const auto saved = ctx->get_saved_variables();
+    const at::Tensor &qkv = saved[0], &out = saved[1], &lse = saved[2];
+    c10::cuda::CUDAGuard guard(qkv.device());
+    const int64_t B = out.size(0), D = out.size(3);
+    const Shape s = shape_of(B, out.size(1), out.size(2), out.size(2), D, ctx->saved_data["window"].toInt(),
+                             ctx->saved_data["sinks"].toInt());
+    at::Tensor dqkv = at::empty(qkv.sizes(), qkv.options());
+    attn_window::backward(grads[0], part_of(qkv, 0, D), part_of(qkv, 1, D), part_of(qkv, 2, D), out, lse,
+                          part_of(dqkv, 0, D), part_of(dqkv, 1, D), part_of(dqkv, 2, D), B, s);
+    debug_check("window_attention backward");
+    return {dqkv, at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor()};
+  }
+};
 
 }  // namespace attn_window
 }  // namespace dst
 
 using namespace dst;
 
-// q [B, T, H, D], k and v [B, T, Hk, D] -> out [B, T, H, D] (contiguous) and the
-// base-2 log-sum-exp [B, H, T rounded up to 128].
-std::vector<at::Tensor> window_attn_fwd(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, int64_t window,
-                                        int64_t sinks) {
-  using namespace attn_window;
-  check_operand(q, "q");
-  check_operand(k, "k");
-  check_operand(v, "v");
-  TORCH_CHECK(k.sizes() == v.sizes() && k.size(0) == q.size(0) && k.size(1) == q.size(1) && k.size(3) == q.size(3),
+// q [B, T, H, D], k and v [B, T, Hk, D], any strides -> [B, T, H, D], differentiable.
+at::Tensor window_attention_qkv(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, int64_t window,
+                                int64_t sinks) {
+  attn_window::check_bf16(q, "q");
+  attn_window::check_bf16(k, "k");
+  attn_window::check_bf16(v, "v");
+  TORCH_CHECK(q.dim() == 4 && k.dim() == 4 && k.sizes() == v.sizes() && k.size(0) == q.size(0) &&
+                  k.size(1) == q.size(1) && k.size(3) == q.size(3),
               "window attention: q [B, T, H, D] and k, v [B, T, Hk, D] must agree");
   TORCH_CHECK(k.device() == q.device() && v.device() == q.device(), "window attention: q, k, v on one device");
-  c10::cuda::CUDAGuard guard(q.device());
-  const Shape s = shape_of(q, k, window, sinks);
-  at::Tensor out = at::empty({q.size(0), q.size(1), q.size(2), q.size(3)}, q.options());
-  at::Tensor lse = at::empty({q.size(0), q.size(2), s.Tp}, q.options().dtype(at::kFloat));
-  if (s.D <= 64)
-    run_fwd<64>(q, k, v, out, lse, s);
-  else
-    run_fwd<128>(q, k, v, out, lse, s);
-  return {out, lse};
+  return attn_window::SeparateFn::apply(q, k, v, window, sinks);
 }
 
-// Gradients into dq, dk, dv (any layout that q, k, v may have).
-void window_attn_bwd(const at::Tensor& dout, const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
-                     const at::Tensor& out, const at::Tensor& lse, const at::Tensor& dq, const at::Tensor& dk,
-                     const at::Tensor& dv, int64_t window, int64_t sinks) {
-  using namespace attn_window;
-  const std::pair<const at::Tensor*, const char*> operands[] = {{&q, "q"},       {&k, "k"},   {&v, "v"},   {&dout, "dout"},
-                                                                {&out, "out"},   {&dq, "dq"}, {&dk, "dk"}, {&dv, "dv"}};
-  for (const auto& [x, name] : operands) {
-    check_operand(*x, name);
-    TORCH_CHECK(x->device() == q.device(), "window attention bwd: ", name, " on another device than q");
-  }
-  TORCH_CHECK(k.sizes() == v.sizes() && k.size(0) == q.size(0) && k.size(1) == q.size(1) && k.size(3) == q.size(3),
-              "window attention bwd: q [B, T, H, D] and k, v [B, T, Hk, D] must agree");
-  TORCH_CHECK(dq.sizes() == q.sizes() && dk.sizes() == k.sizes() && dv.sizes() == v.sizes(),
-              "window attention bwd: gradients shaped like q, k, v required");
-  TORCH_CHECK(out.is_contiguous() && dout.is_contiguous() && out.sizes() == q.sizes() && dout.sizes() == q.sizes(),
-              "window attention bwd: contiguous out and dout shaped like q required");
-  c10::cuda::CUDAGuard guard(q.device());
-  const Shape s = shape_of(q, k, window, sinks);
-  TORCH_CHECK(lse.is_cuda() && lse.device() == q.device() && lse.is_contiguous() && lse.scalar_type() == at::kFloat &&
-                  lse.dim() == 3 && lse.size(0) == q.size(0) && lse.size(1) == q.size(2) && lse.size(2) == s.Tp,
-              "window attention bwd: lse as the forward pass returned it required");
-  at::Tensor di = at::empty_like(lse);
-  if (s.D <= 64)
-    run_bwd<64>(dout, q, k, v, out, lse, di, dq, dk, dv, s);
-  else
-    run_bwd<128>(dout, q, k, v, out, lse, di, dq, dk, dv, s);
+// qkv [B, T, n_head * 3 * head_dim] -> [B, T, n_head * head_dim], differentiable.
+at::Tensor window_attention(const at::Tensor& qkv, int64_t n_head, int64_t head_dim, int64_t window, int64_t sinks) {
+  attn_window::check_bf16(qkv, "qkv");
+  TORCH_CHECK(qkv.dim() == 3 && n_head >= 1 && head_dim >= 1 && qkv.size(2) == 3 * n_head * head_dim,
+              "window attention: qkv must be [B, T, n_head * 3 * head_dim]");
+  return attn_window::FusedFn::apply(qkv, n_head, head_dim, window, sinks);
 }
 
 void register_attn_window(pybind11::module& m) {
-  m.def("window_attn_fwd", &window_attn_fwd, "sliding-window attention with sinks, forward", pybind11::arg("q"),
+  m.def("window_attention_qkv", &window_attention_qkv, "sliding-window attention with sinks", pybind11::arg("q"),
         pybind11::arg("k"), pybind11::arg("v"), pybind11::arg("window"), pybind11::arg("sinks"));
-  m.def("window_attn_bwd", &window_attn_bwd, "sliding-window attention with sinks, backward", pybind11::arg("dout"),
-        pybind11::arg("q"), pybind11::arg("k"), pybind11::arg("v"), pybind11::arg("out"), pybind11::arg("lse"),
-        pybind11::arg("dq"), pybind11::arg("dk"), pybind11::arg("dv"), pybind11::arg("window"), pybind11::arg("sinks"));
+  m.def("window_attention", &window_attention, "sliding-window attention with sinks over a fused qkv buffer",
+        pybind11::arg("qkv"), pybind11::arg("n_head"), pybind11::arg("head_dim"), pybind11::arg("window"),
+        pybind11::arg("sinks"));
 }

@@ -2,7 +2,9 @@
 #include <c10/cuda/CUDAGuard.h>
 #include <cuda_runtime.h>
 
+#include <cstdlib>
 #include <mutex>
+#include <string>
 
 #include "common.h"
 
@@ -19,6 +21,16 @@ int* status_ptr() {
     C10_CUDA_CHECK(cudaMemset(ptrs[dev], 0, sizeof(int)));
   }
   return ptrs[dev];
+}
+
+void debug_check(const char* op) {
+  const char* on = std::getenv("DST_DEBUG_SYNC");
+  if (on == nullptr || *on == '\0' || std::string(on) == "0") return;
+  int code = 0;
+  C10_CUDA_CHECK(cudaDeviceSynchronize());
+  C10_CUDA_CHECK(cudaMemcpy(&code, status_ptr(), sizeof(int), cudaMemcpyDeviceToHost));
+  C10_CUDA_CHECK(cudaMemset(status_ptr(), 0, sizeof(int)));
+  TORCH_CHECK(code == 0, "native op '", op, "' reported status ", std::to_string(code));
 }
 
 }  // namespace dst

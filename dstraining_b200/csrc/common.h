@@ -15,6 +15,10 @@ int* status_ptr();
 
 int num_sms();
 
+// With DST_DEBUG_SYNC set: wait for the device and raise if a kernel of `op`
+// left an error in the status word.
+void debug_check(const char* op);
+
 CUtensorMap make_tmap_bf16(const void* base, uint64_t inner, uint64_t outer, uint64_t ld, uint32_t box_inner,
                            uint32_t box_outer);
 

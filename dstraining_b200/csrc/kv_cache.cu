@@ -30,6 +30,9 @@
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/extension.h>
 
+#include <map>
+#include <string>
+
 #include "common.h"
 #include "ptx.cuh"
 
@@ -760,243 +763,225 @@ __global__ void __launch_bounds__(kThreads, StepCfg<DP, BITS>::kCtas)
 }
 
 // -------------------------------------------------------------------- host
-int padded_dim(int64_t D) { return D <= 64 ? 64 : 128; }
+// Operands the kernels can address as they are: unit inner stride, other strides
+// and the start multiples of 16 bytes. Anything else is copied.
+at::Tensor as_rows(const at::Tensor& x) {
+  bool ok = x.stride(-1) == 1 && reinterpret_cast<uintptr_t>(x.data_ptr()) % 16 == 0;
+  for (int i = 0; i + 1 < x.dim(); ++i) ok = ok && (x.size(i) == 1 || x.stride(i) % 8 == 0);
+  return ok ? x : x.clone(at::MemoryFormat::Contiguous);
+}
 
-struct Cache {  // the tensors of one cache, checked
-  int64_t B, Hk, alloc, D;
-  int DP, bits;
-  Store ks, vs;
+std::string sizes_text(at::IntArrayRef x) {
+  std::string s = "[";
+  for (size_t i = 0; i < x.size(); ++i) s += (i ? ", " : "") + std::to_string(x[i]);
+  return s + "]";
+}
+
+// The rows of one layer's cache and what a step over them needs.
+class KVCache {
+ public:
+  KVCache(int64_t batch, int64_t kv_heads, int64_t head_dim, int64_t window, int64_t sinks, int64_t bits, at::Tensor pos)
+      : B_(batch), Hk_(kv_heads), D_(head_dim), bits_(static_cast<int>(bits)), pos_(std::move(pos)) {
+    TORCH_CHECK_VALUE(D_ >= 8 && D_ <= 128 && D_ % 8 == 0 && (bits == 16 || (bits == 4 && D_ % 32 == 0)),
+                      "kv cache: the CUDA cache takes head sizes that are multiples of 8 up to 128 (of 32 in 4 bits), got ",
+                      std::to_string(D_));
+    TORCH_CHECK_VALUE(window >= 1 && sinks >= 0 && window < (int64_t(1) << 31) && sinks < (int64_t(1) << 31),
+                      "kv cache: window >= 1 and sinks >= 0 required");
+    slots_ = window + sinks;
+    DP_ = D_ <= 64 ? 64 : 128;
+    const int64_t alloc = (slots_ + 63) / 64 * 64;  // whole tiles; rows past the last slot are never visible
+    TORCH_CHECK_VALUE(B_ >= 1 && B_ <= 65535 && Hk_ >= 1 && Hk_ <= 32767 && alloc < (int64_t(1) << 31) / (B_ * Hk_),
+                      "kv cache: batch, heads or slots out of range (2^31 rows at most)");
+    check_positions(pos_, "pos");
+    ring_ = {window, sinks, static_cast<int>(alloc)};
+    c10::cuda::CUDAGuard guard(pos_.device());
+    const auto options = pos_.options();
+    for (int i = 0; i < 2; ++i) {
+      rows_[i] = bits == 16 ? at::zeros({B_, Hk_, alloc, DP_}, options.dtype(at::kBFloat16))
+                            : at::zeros({B_, Hk_, alloc, DP_ / 2}, options.dtype(at::kByte));
+      if (bits == 4) params_[i] = at::zeros({B_, Hk_, alloc, DP_ / 32}, options.dtype(at::kInt));
+      store_[i] = {static_cast<uint8_t*>(rows_[i].data_ptr()),
+                   bits == 4 ? static_cast<uint32_t*>(params_[i].data_ptr()) : nullptr};
+    }
+    dispatch([&](auto dp, auto bits_c) {
+      if constexpr (bits_c() == 16) {
+        const uint64_t n = static_cast<uint64_t>(B_) * Hk_ * alloc;
+        for (int i = 0; i < 2; ++i)
+          map_[i] = make_tmap_bf16(rows_[i].data_ptr(), dp(), n, dp(), 64, StepCfg<dp(), 16>::KT);
+      }
+    });
+  }
+
+  // k, v [B, T, Hk, D]: the visible tokens of each prompt; pos[b] = its length.
+  void fill(const at::Tensor& k_, const at::Tensor& v_, const c10::optional<at::Tensor>& lengths) {
+    TORCH_CHECK_VALUE(k_.dim() == 4, "k must be [B, T, Hk, D], got ", sizes_text(k_.sizes()));
+    const int64_t T = k_.size(1);
+    TORCH_CHECK_VALUE(T < (int64_t(1) << 31), "kv cache: prompt too long");
+    check_rows(k_, {B_, T, Hk_, D_}, "k");
+    check_rows(v_, {B_, T, Hk_, D_}, "v");
+    if (lengths) check_positions(*lengths, "lengths");
+    c10::cuda::CUDAGuard guard(pos_.device());
+    if (T == 0) {
+      pos_.zero_();
+      return;
+    }
+    const at::Tensor k = as_rows(k_), v = as_rows(v_);
+    const int rows = static_cast<int>(std::min<int64_t>(T, slots_));
+    const View kv = {static_cast<const __nv_bfloat16*>(k.data_ptr()), k.stride(0), k.stride(2), k.stride(1)};
+    const View vv = {static_cast<const __nv_bfloat16*>(v.data_ptr()), v.stride(0), v.stride(2), v.stride(1)};
+    dispatch([&](auto dp, auto bits) {
+      const dim3 grid(static_cast<unsigned>((static_cast<int64_t>(rows) * (dp() / 8) + 255) / 256),
+                      static_cast<unsigned>(2 * Hk_), static_cast<unsigned>(B_));
+      fill_kernel<dp(), bits()><<<grid, 256, 0, at::cuda::getCurrentCUDAStream()>>>(
+          kv, vv, lengths ? lengths->data_ptr<int64_t>() : nullptr, pos_.data_ptr<int64_t>(), store_[0], store_[1],
+          ring_, static_cast<int>(T), rows, static_cast<int>(Hk_), static_cast<int>(D_), status_ptr());
+    });
+    C10_CUDA_KERNEL_LAUNCH_CHECK();
+    debug_check("kv_cache fill");
+  }
+
+  // The held rows [B, Hk, slots, D] in slot order: bf16, or fp32 for 4 bits.
+  std::pair<at::Tensor, at::Tensor> read() {
+    c10::cuda::CUDAGuard guard(pos_.device());
+    const auto options = pos_.options().dtype(bits_ == 16 ? at::kBFloat16 : at::kFloat);
+    at::Tensor k = at::empty({B_, Hk_, slots_, D_}, options), v = at::empty({B_, Hk_, slots_, D_}, options);
+    dispatch([&](auto dp, auto bits) {
+      const dim3 grid(static_cast<unsigned>((slots_ * (dp() / 8) + 255) / 256), static_cast<unsigned>(2 * Hk_),
+                      static_cast<unsigned>(B_));
+      read_kernel<dp(), bits()><<<grid, 256, 0, at::cuda::getCurrentCUDAStream()>>>(
+          store_[0], store_[1], pos_.data_ptr<int64_t>(), k.data_ptr(), v.data_ptr(), ring_, static_cast<int>(slots_),
+          static_cast<int>(Hk_), static_cast<int>(D_));
+    });
+    C10_CUDA_KERNEL_LAUNCH_CHECK();
+    debug_check("kv_cache read");
+    return {k, v};
+  }
+
+  // One token per sequence: q [B, H, D], k and v [B, Hk, D], pos [B] (-1: idle).
+  // The attention [B, H, D] over the cache with the token in it and, on request,
+  // what the stored rows stand for (fp32 [B, Hk, D]).
+  std::vector<at::Tensor> step(const at::Tensor& q_, const at::Tensor& k_, const at::Tensor& v_, const at::Tensor& pos,
+                               bool return_stored) {
+    TORCH_CHECK_VALUE(q_.dim() == 3 && q_.size(1) >= 1 && q_.size(1) % Hk_ == 0, "q must be [B, H, D] with H a multiple of ",
+                      std::to_string(Hk_), ", got ", sizes_text(q_.sizes()));
+    const int64_t H = q_.size(1), G = H / Hk_, chunks = (G + kRows - 1) / kRows;
+    check_rows(q_, {B_, H, D_}, "q");
+    check_rows(k_, {B_, Hk_, D_}, "k");
+    check_rows(v_, {B_, Hk_, D_}, "v");
+    check_positions(pos, "pos");
+    TORCH_CHECK_VALUE(Hk_ * chunks <= 65535, "kv cache: too many query heads");
+    c10::cuda::CUDAGuard guard(pos_.device());
+    const at::Tensor q = as_rows(q_), k = as_rows(k_), v = as_rows(v_);
+    const Work& work = work_for(chunks);
+    at::Tensor out = at::empty({B_, H, D_}, q.options());
+    std::vector<at::Tensor> result = {out};
+    StepArgs a;
+    a.q = static_cast<const __nv_bfloat16*>(q.data_ptr());
+    a.q_b = q.stride(0), a.q_h = q.stride(1);
+    a.k = {static_cast<const __nv_bfloat16*>(k.data_ptr()), k.stride(0), k.stride(1), 0};
+    a.v = {static_cast<const __nv_bfloat16*>(v.data_ptr()), v.stride(0), v.stride(1), 0};
+    a.pos = pos.data_ptr<int64_t>();
+    a.ks = store_[0], a.vs = store_[1];
+    a.out = static_cast<__nv_bfloat16*>(out.data_ptr());
+    a.stored_k = a.stored_v = nullptr;
+    if (return_stored) {
+      for (int i = 0; i < 2; ++i) result.push_back(at::empty({B_, Hk_, D_}, q.options().dtype(at::kFloat)));
+      a.stored_k = result[1].data_ptr<float>();
+      a.stored_v = result[2].data_ptr<float>();
+    }
+    a.partial = work.partial.data_ptr<float>();
+    a.arrived = work.arrived.data_ptr<int>();
+    a.ring = ring_;
+    a.slots = static_cast<int>(slots_), a.Hk = static_cast<int>(Hk_), a.G = static_cast<int>(G);
+    a.D = static_cast<int>(D_), a.chunks = static_cast<int>(chunks), a.splits = work.splits;
+    a.scale_log2 = static_cast<float>(1.4426950408889634 / std::sqrt(static_cast<double>(D_)));
+    a.status = status_ptr();
+    const dim3 grid(static_cast<unsigned>(work.splits), static_cast<unsigned>(Hk_ * chunks), static_cast<unsigned>(B_));
+    dispatch([&](auto dp, auto bits) {
+      using C = StepCfg<dp(), bits()>;
+      auto kernel = step_kernel<dp(), bits()>;
+      static bool configured[64] = {false};
+      const int dev = pos_.device().index();
+      if (!configured[dev])
+        C10_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem));
+      configured[dev] = true;
+      kernel<<<grid, kThreads, C::kSmem, at::cuda::getCurrentCUDAStream()>>>(map_[0], map_[1], a);
+    });
+    C10_CUDA_KERNEL_LAUNCH_CHECK();
+    debug_check("kv_cache step");
+    return result;
+  }
+
+  const at::Tensor& rows(int i) const { return rows_[i]; }
+  const at::Tensor& params(int i) const { return params_[i]; }
+
+ private:
+  struct Work {  // joining the CTAs that share a cache; the counters are 0 between launches
+    int splits;
+    at::Tensor partial, arrived;
+  };
+
+  template <typename F>
+  void dispatch(F&& f) const {
+    using std::integral_constant;
+    if (DP_ == 64 && bits_ == 16) f(integral_constant<int, 64>(), integral_constant<int, 16>());
+    if (DP_ == 64 && bits_ == 4) f(integral_constant<int, 64>(), integral_constant<int, 4>());
+    if (DP_ == 128 && bits_ == 16) f(integral_constant<int, 128>(), integral_constant<int, 16>());
+    if (DP_ == 128 && bits_ == 4) f(integral_constant<int, 128>(), integral_constant<int, 4>());
+  }
+
+  // How many CTAs share the slots of one (sequence, key head): enough to fill the
+  // GPU, each with at least one tile per warp.
+  const Work& work_for(int64_t chunks) {
+    auto it = work_.find(chunks);
+    if (it != work_.end()) return it->second;
+    const int64_t units = B_ * Hk_ * chunks;
+    int64_t splits = 1;
+    dispatch([&](auto dp, auto bits) {
+      using C = StepCfg<dp(), bits()>;
+      const int64_t most = (slots_ + kWarps * C::KT - 1) / (kWarps * C::KT);
+      splits = std::min(most, std::max<int64_t>(1, (C::kCtas * num_sms() + units - 1) / units));
+    });
+    Work w = {static_cast<int>(splits), at::empty({units * splits * kRows * (DP_ + 2)}, pos_.options().dtype(at::kFloat)),
+              at::zeros({units}, pos_.options().dtype(at::kInt))};
+    return work_.emplace(chunks, std::move(w)).first->second;
+  }
+
+  void check_rows(const at::Tensor& x, std::initializer_list<int64_t> sizes, const char* name) const {
+    TORCH_CHECK_VALUE(x.sizes() == at::IntArrayRef(sizes) && x.scalar_type() == at::kBFloat16 && x.device() == pos_.device(),
+                      name, " must be a bf16 tensor ", sizes_text(at::IntArrayRef(sizes)), " on the cache's device, got ",
+                      sizes_text(x.sizes()), " ", c10::toString(x.scalar_type()));
+  }
+
+  void check_positions(const at::Tensor& x, const char* name) const {
+    TORCH_CHECK_VALUE(x.is_cuda() && (!pos_.defined() || x.device() == pos_.device()) && x.scalar_type() == at::kLong &&
+                          x.is_contiguous() && x.dim() == 1 && x.size(0) == B_,
+                      name, " must be a contiguous int64 tensor [", std::to_string(B_), "] on the cache's device");
+  }
+
+  int64_t B_, Hk_, D_, slots_, DP_;
+  int bits_;
+  at::Tensor pos_, rows_[2], params_[2];
+  Store store_[2];
+  Ring ring_;
+  CUtensorMap map_[2] = {};
+  std::map<int64_t, Work> work_;
 };
-
-Cache check_cache(const at::Tensor& keys, const at::Tensor& values, const c10::optional<at::Tensor>& key_params,
-                  const c10::optional<at::Tensor>& value_params, int64_t D, int64_t slots) {
-  Cache c;
-  TORCH_CHECK(D >= 8 && D <= 128 && D % 8 == 0, "kv cache: head_dim must be a multiple of 8 up to 128, got ",
-              std::to_string(D));
-  c.D = D;
-  c.DP = padded_dim(D);
-  c.bits = keys.scalar_type() == at::kBFloat16 ? 16 : 4;
-  TORCH_CHECK(c.bits == 16 || (keys.scalar_type() == at::kByte && D % 32 == 0),
-              "kv cache: bf16 rows, or uint8 rows with head_dim a multiple of 32");
-  const int64_t row = c.bits == 16 ? c.DP : c.DP / 2;
-  for (const at::Tensor* x : {&keys, &values})
-    TORCH_CHECK(x->is_cuda() && x->is_contiguous() && x->dim() == 4 && x->size(3) == row &&
-                    x->scalar_type() == keys.scalar_type() && x->sizes() == keys.sizes() &&
-                    x->device() == keys.device() && reinterpret_cast<uintptr_t>(x->data_ptr()) % 16 == 0,
-                "kv cache: contiguous, aligned keys and values [B, Hk, slots, ", std::to_string(row), "] required");
-  c.B = keys.size(0);
-  c.Hk = keys.size(1);
-  c.alloc = keys.size(2);
-  TORCH_CHECK(c.alloc % 64 == 0 && slots >= 1 && slots <= c.alloc, "kv cache: slots in whole tiles of 64 required");
-  TORCH_CHECK(c.B >= 1 && c.B <= 65535 && c.Hk >= 1 && c.Hk <= 32767, "kv cache: batch or heads out of range");
-  TORCH_CHECK(c.B * c.Hk * c.alloc < (int64_t(1) << 31), "kv cache: more than 2^31 rows");
-  c.ks = {static_cast<uint8_t*>(keys.data_ptr()), nullptr};
-  c.vs = {static_cast<uint8_t*>(values.data_ptr()), nullptr};
-  if (c.bits == 4) {
-    TORCH_CHECK(key_params.has_value() && value_params.has_value(), "kv cache: 4-bit rows need their parameters");
-    for (const at::Tensor* x : {&*key_params, &*value_params})
-      TORCH_CHECK(x->is_cuda() && x->is_contiguous() && x->scalar_type() == at::kInt && x->dim() == 4 &&
-                      x->size(0) == c.B && x->size(1) == c.Hk && x->size(2) == c.alloc && x->size(3) == c.DP / 32 &&
-                      x->device() == keys.device() && reinterpret_cast<uintptr_t>(x->data_ptr()) % 16 == 0,
-                  "kv cache: contiguous int32 parameters [B, Hk, slots, ", std::to_string(c.DP / 32), "] required");
-    c.ks.params = reinterpret_cast<uint32_t*>(key_params->data_ptr());
-    c.vs.params = reinterpret_cast<uint32_t*>(value_params->data_ptr());
-  }
-  return c;
-}
-
-Ring ring_of(const Cache& c, int64_t window, int64_t sinks, int64_t slots) {
-  TORCH_CHECK(window >= 1 && sinks >= 0 && window + sinks == slots, "kv cache: window + sinks must be the slots");
-  return {window, sinks, static_cast<int>(c.alloc)};
-}
-
-void check_rows(const at::Tensor& x, const Cache& c, const at::Tensor& keys, const char* name) {
-  TORCH_CHECK(x.is_cuda() && x.device() == keys.device() && x.scalar_type() == at::kBFloat16 && x.stride(-1) == 1 &&
-                  reinterpret_cast<uintptr_t>(x.data_ptr()) % 16 == 0 && x.size(0) == c.B && x.size(-1) == c.D,
-              "kv cache: ", name, " must be CUDA bf16 with unit inner stride, 16-byte aligned, of the cache's batch "
-              "and head_dim");
-  for (int i = 0; i + 1 < x.dim(); ++i)
-    TORCH_CHECK(x.size(i) == 1 || x.stride(i) % 8 == 0, "kv cache: ", name, " strides must be multiples of 8 elements");
-}
-
-void check_positions(const at::Tensor& x, const Cache& c, const at::Tensor& keys, const char* name) {
-  TORCH_CHECK(x.is_cuda() && x.device() == keys.device() && x.scalar_type() == at::kLong && x.is_contiguous() &&
-                  x.dim() == 1 && x.size(0) == c.B,
-              "kv cache: ", name, " must be a contiguous CUDA int64 tensor [B]");
-}
-
-template <typename F>
-void dispatch(const Cache& c, F&& f) {
-  if (c.DP == 64) {
-    if (c.bits == 16)
-      f(std::integral_constant<int, 64>(), std::integral_constant<int, 16>());
-    else
-      f(std::integral_constant<int, 64>(), std::integral_constant<int, 4>());
-  } else {
-    if (c.bits == 16)
-      f(std::integral_constant<int, 128>(), std::integral_constant<int, 16>());
-    else
-      f(std::integral_constant<int, 128>(), std::integral_constant<int, 4>());
-  }
-}
 
 }  // namespace kv_cache
 }  // namespace dst
 
 using namespace dst;
 
-using OptTensor = c10::optional<at::Tensor>;
-
-// k, v [B, T, Hk, D]: the visible tokens of each prompt into the cache; pos[b] = its length.
-void kv_cache_fill(const at::Tensor& k, const at::Tensor& v, const OptTensor& lengths, const at::Tensor& pos,
-                   const at::Tensor& keys, const at::Tensor& values, const OptTensor& key_params,
-                   const OptTensor& value_params, int64_t window, int64_t sinks) {
-  using namespace kv_cache;
-  const int64_t slots = window + sinks;
-  TORCH_CHECK(k.dim() == 4 && v.dim() == 4 && k.sizes() == v.sizes(), "kv cache: k and v [B, T, Hk, D] required");
-  const Cache c = check_cache(keys, values, key_params, value_params, k.size(3), slots);
-  const Ring ring = ring_of(c, window, sinks, slots);
-  check_rows(k, c, keys, "k");
-  check_rows(v, c, keys, "v");
-  TORCH_CHECK(k.size(2) == c.Hk, "kv cache: k and v must have the cache's heads");
-  TORCH_CHECK(k.size(1) >= 1 && k.size(1) < (int64_t(1) << 31), "kv cache: prompt length out of range");
-  if (lengths) check_positions(*lengths, c, keys, "lengths");
-  check_positions(pos, c, keys, "pos");
-  c10::cuda::CUDAGuard guard(keys.device());
-  const int T = static_cast<int>(k.size(1));
-  const int rows = static_cast<int>(std::min<int64_t>(T, slots));
-  const View kv = {static_cast<const __nv_bfloat16*>(k.data_ptr()), k.stride(0), k.stride(2), k.stride(1)};
-  const View vv = {static_cast<const __nv_bfloat16*>(v.data_ptr()), v.stride(0), v.stride(2), v.stride(1)};
-  dispatch(c, [&](auto dp, auto bits) {
-    const int64_t threads = static_cast<int64_t>(rows) * (dp() / 8);
-    const dim3 grid(static_cast<unsigned>((threads + 255) / 256), static_cast<unsigned>(2 * c.Hk), static_cast<unsigned>(c.B));
-    fill_kernel<dp(), bits()><<<grid, 256, 0, at::cuda::getCurrentCUDAStream()>>>(
-        kv, vv, lengths ? lengths->data_ptr<int64_t>() : nullptr, pos.data_ptr<int64_t>(), c.ks, c.vs, ring, T, rows,
-        static_cast<int>(c.Hk), static_cast<int>(c.D), status_ptr());
-  });
-  C10_CUDA_KERNEL_LAUNCH_CHECK();
-}
-
-// The held rows [B, Hk, slots, D] in slot order: bf16, or fp32 for 4 bits.
-std::vector<at::Tensor> kv_cache_read(const at::Tensor& pos, const at::Tensor& keys, const at::Tensor& values,
-                                      const OptTensor& key_params, const OptTensor& value_params, int64_t window,
-                                      int64_t sinks, int64_t D) {
-  using namespace kv_cache;
-  const int64_t slots = window + sinks;
-  const Cache c = check_cache(keys, values, key_params, value_params, D, slots);
-  const Ring ring = ring_of(c, window, sinks, slots);
-  check_positions(pos, c, keys, "pos");
-  c10::cuda::CUDAGuard guard(keys.device());
-  auto options = keys.options().dtype(c.bits == 16 ? at::kBFloat16 : at::kFloat);
-  at::Tensor ko = at::empty({c.B, c.Hk, slots, D}, options), vo = at::empty({c.B, c.Hk, slots, D}, options);
-  dispatch(c, [&](auto dp, auto bits) {
-    const int64_t threads = slots * (dp() / 8);
-    const dim3 grid(static_cast<unsigned>((threads + 255) / 256), static_cast<unsigned>(2 * c.Hk), static_cast<unsigned>(c.B));
-    read_kernel<dp(), bits()><<<grid, 256, 0, at::cuda::getCurrentCUDAStream()>>>(
-        c.ks, c.vs, pos.data_ptr<int64_t>(), ko.data_ptr(), vo.data_ptr(), ring, static_cast<int>(slots),
-        static_cast<int>(c.Hk), static_cast<int>(D));
-  });
-  C10_CUDA_KERNEL_LAUNCH_CHECK();
-  return {ko, vo};
-}
-
-// How many CTAs share the slots of one (sequence, key head), and the floats and
-// counters that joining them takes: enough CTAs to fill the GPU, each with at
-// least one tile per warp.
-std::vector<int64_t> kv_cache_plan(int64_t batch, int64_t kv_heads, int64_t heads, int64_t D, int64_t slots, bool packed) {
-  using namespace kv_cache;
-  TORCH_CHECK(batch >= 1 && kv_heads >= 1 && heads >= 1 && heads % kv_heads == 0 && slots >= 1,
-              "kv cache: query heads must be a multiple of the key heads");
-  const int64_t chunks = (heads / kv_heads + kRows - 1) / kRows, units = batch * kv_heads * chunks;
-  const int DP = padded_dim(D);
-  const int64_t tile = packed ? (DP == 64 ? 64 : 32) : (DP == 64 ? 32 : 16);
-  const int64_t ctas = packed ? (DP == 64 ? 4 : 3) : 2;
-  const int64_t most = std::max<int64_t>(1, (slots + kWarps * tile - 1) / (kWarps * tile));
-  const int64_t splits = std::min(most, std::max<int64_t>(1, (ctas * num_sms() + units - 1) / units));
-  return {splits, units * splits * kRows * (DP + 2), units};
-}
-
-// One token per sequence: q [B, H, D], k and v [B, Hk, D], pos [B] (-1: idle).
-// Returns the attention [B, H, D] over the cache with the token in it, and (on
-// request) what the stored rows stand for, fp32 [B, Hk, D].
-std::vector<at::Tensor> kv_cache_step(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
-                                      const at::Tensor& pos, const at::Tensor& keys, const at::Tensor& values,
-                                      const OptTensor& key_params, const OptTensor& value_params,
-                                      const at::Tensor& partial, const at::Tensor& arrived, int64_t window,
-                                      int64_t sinks, int64_t splits, bool return_stored) {
-  using namespace kv_cache;
-  const int64_t slots = window + sinks;
-  TORCH_CHECK(q.dim() == 3 && k.dim() == 3 && v.dim() == 3 && k.sizes() == v.sizes(),
-              "kv cache: q [B, H, D] and k, v [B, Hk, D] required");
-  const Cache c = check_cache(keys, values, key_params, value_params, q.size(2), slots);
-  const Ring ring = ring_of(c, window, sinks, slots);
-  check_rows(q, c, keys, "q");
-  check_rows(k, c, keys, "k");
-  check_rows(v, c, keys, "v");
-  check_positions(pos, c, keys, "pos");
-  TORCH_CHECK(k.size(1) == c.Hk && q.size(1) >= 1 && q.size(1) % c.Hk == 0,
-              "kv cache: query heads must be a multiple of the cache's heads");
-  const int64_t H = q.size(1), G = H / c.Hk, chunks = (G + kRows - 1) / kRows, units = c.B * c.Hk * chunks;
-  TORCH_CHECK(c.Hk * chunks <= 65535, "kv cache: too many heads");
-  TORCH_CHECK(splits >= 1 && splits <= 65535 && partial.is_cuda() && partial.device() == keys.device() &&
-                  partial.is_contiguous() && partial.scalar_type() == at::kFloat &&
-                  partial.numel() >= units * splits * kRows * (c.DP + 2) && arrived.is_cuda() &&
-                  arrived.device() == keys.device() && arrived.is_contiguous() &&
-                  arrived.scalar_type() == at::kInt && arrived.numel() >= units,
-              "kv cache: workspace too small for this call");
-  c10::cuda::CUDAGuard guard(keys.device());
-  at::Tensor out = at::empty({c.B, H, c.D}, q.options());
-  std::vector<at::Tensor> result = {out};
-  StepArgs a;
-  a.q = static_cast<const __nv_bfloat16*>(q.data_ptr());
-  a.q_b = q.stride(0), a.q_h = q.stride(1);
-  a.k = {static_cast<const __nv_bfloat16*>(k.data_ptr()), k.stride(0), k.stride(1), 0};
-  a.v = {static_cast<const __nv_bfloat16*>(v.data_ptr()), v.stride(0), v.stride(1), 0};
-  a.pos = pos.data_ptr<int64_t>();
-  a.ks = c.ks, a.vs = c.vs;
-  a.out = static_cast<__nv_bfloat16*>(out.data_ptr());
-  a.stored_k = a.stored_v = nullptr;
-  if (return_stored) {
-    for (int i = 0; i < 2; ++i) result.push_back(at::empty({c.B, c.Hk, c.D}, q.options().dtype(at::kFloat)));
-    a.stored_k = result[1].data_ptr<float>();
-    a.stored_v = result[2].data_ptr<float>();
-  }
-  a.partial = partial.data_ptr<float>();
-  a.arrived = arrived.data_ptr<int>();
-  a.ring = ring;
-  a.slots = static_cast<int>(slots), a.Hk = static_cast<int>(c.Hk), a.G = static_cast<int>(G);
-  a.D = static_cast<int>(c.D), a.chunks = static_cast<int>(chunks), a.splits = static_cast<int>(splits);
-  a.scale_log2 = static_cast<float>(1.4426950408889634 / std::sqrt(static_cast<double>(c.D)));
-  a.status = status_ptr();
-  const dim3 grid(static_cast<unsigned>(splits), static_cast<unsigned>(c.Hk * chunks), static_cast<unsigned>(c.B));
-  dispatch(c, [&](auto dp, auto bits) {
-    using C = StepCfg<dp(), bits()>;
-    CUtensorMap tk{}, tv{};
-    if (bits() == 16) {
-      const uint64_t rows = static_cast<uint64_t>(c.B) * c.Hk * c.alloc;
-      tk = make_tmap_bf16(keys.data_ptr(), dp(), rows, dp(), 64, C::KT);
-      tv = make_tmap_bf16(values.data_ptr(), dp(), rows, dp(), 64, C::KT);
-    }
-    auto kernel = step_kernel<dp(), bits()>;
-    C10_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem));
-    kernel<<<grid, kThreads, C::kSmem, at::cuda::getCurrentCUDAStream()>>>(tk, tv, a);
-  });
-  C10_CUDA_KERNEL_LAUNCH_CHECK();
-  return result;
-}
-
 void register_kv_cache(pybind11::module& m) {
   namespace py = pybind11;
-  m.def("kv_cache_fill", &kv_cache_fill, "prompt rows into a rolling key/value cache", py::arg("k"), py::arg("v"),
-        py::arg("lengths"), py::arg("pos"), py::arg("keys"), py::arg("values"), py::arg("key_params"),
-        py::arg("value_params"), py::arg("window"), py::arg("sinks"));
-  m.def("kv_cache_read", &kv_cache_read, "held rows of a rolling key/value cache", py::arg("pos"), py::arg("keys"),
-        py::arg("values"), py::arg("key_params"), py::arg("value_params"), py::arg("window"), py::arg("sinks"),
-        py::arg("D"));
-  m.def("kv_cache_plan", &kv_cache_plan, "splits, partial floats and counters of a step", py::arg("batch"),
-        py::arg("kv_heads"), py::arg("heads"), py::arg("D"), py::arg("slots"), py::arg("packed"));
-  m.def("kv_cache_step", &kv_cache_step, "one token per sequence over a rolling key/value cache", py::arg("q"),
-        py::arg("k"), py::arg("v"), py::arg("pos"), py::arg("keys"), py::arg("values"), py::arg("key_params"),
-        py::arg("value_params"), py::arg("partial"), py::arg("arrived"), py::arg("window"), py::arg("sinks"),
-        py::arg("splits"), py::arg("return_stored"));
+  using kv_cache::KVCache;
+  py::class_<KVCache>(m, "KVCache", "rolling key/value cache of one layer (bf16 or 4 bits)")
+      .def(py::init<int64_t, int64_t, int64_t, int64_t, int64_t, int64_t, at::Tensor>(), py::arg("batch"),
+           py::arg("kv_heads"), py::arg("head_dim"), py::arg("window"), py::arg("sinks"), py::arg("bits"), py::arg("pos"))
+      .def("fill", &KVCache::fill, py::arg("k"), py::arg("v"), py::arg("lengths"))
+      .def("read", &KVCache::read)
+      .def("step", &KVCache::step, py::arg("q"), py::arg("k"), py::arg("v"), py::arg("pos"), py::arg("return_stored"))
+      .def("rows", [](const KVCache& c) { return py::make_tuple(c.rows(0), c.rows(1)); })
+      .def("params", [](const KVCache& c) { return py::make_tuple(c.params(0), c.params(1)); });
 }

@@ -48,13 +48,6 @@ def dequantize_rows(code: torch.Tensor, step: torch.Tensor, low: torch.Tensor) -
     return (code.float() * step.float() + low.float()).flatten(-2)
 
 
-def _rows(x: torch.Tensor) -> torch.Tensor:
-    """x itself if the kernels can address it, else a contiguous copy."""
-    ok = x.stride(-1) == 1 and x.data_ptr() % 16 == 0
-    ok = ok and all(x.shape[i] == 1 or x.stride(i) % 8 == 0 for i in range(x.dim() - 1))
-    return x if ok else x.clone(memory_format=torch.contiguous_format)
-
-
 class WindowCache:
     """Keys and values of one layer for ``batch`` sequences.
 
@@ -85,24 +78,14 @@ class WindowCache:
         self.pos = pos if pos is not None else torch.zeros(batch, dtype=torch.int64, device=device)
         if self.pos.shape != (batch,) or self.pos.dtype != torch.int64:
             raise ValueError(f"pos must be an int64 tensor [{batch}]")
-        rows = (batch, n_kv_head)
-        self._params = (None, None)
         if self.native:
-            if head_dim % 8 or head_dim > 128:
-                raise ValueError(f"the CUDA cache takes head sizes that are multiples of 8 up to 128, got {head_dim}")
-            padded = 64 if head_dim <= 64 else 128
-            rows += (-(-self.slots // 64) * 64,)  # whole tiles; the rows past the last slot are never visible
-            if bits == 16:
-                self._rows = tuple(torch.zeros(*rows, padded, dtype=dtype, device=device) for _ in range(2))
-            else:
-                self._rows = tuple(torch.zeros(*rows, padded // 2, dtype=torch.uint8, device=device) for _ in range(2))
-                self._params = tuple(torch.zeros(*rows, padded // GROUP, dtype=torch.int32, device=device)
-                                     for _ in range(2))
-            self._work = {}  # query heads -> (splits, partial results, arrival counters)
+            self._cache = native.lib().KVCache(batch, n_kv_head, head_dim, window, sinks, bits, self.pos)
+            self._rows, self._params = self._cache.rows(), self._cache.params()
         elif bits == 16:
-            self._rows = tuple(torch.zeros(*rows, self.slots, head_dim, dtype=dtype, device=device) for _ in range(2))
+            rows = (batch, n_kv_head, self.slots, head_dim)
+            self._rows = tuple(torch.zeros(rows, dtype=dtype, device=device) for _ in range(2))
         else:
-            groups = rows + (self.slots, head_dim // GROUP)
+            groups = (batch, n_kv_head, self.slots, head_dim // GROUP)
             self._rows = tuple(
                 (torch.zeros(*groups, GROUP, dtype=torch.uint8, device=device),
                  torch.zeros(*groups, 1, dtype=torch.bfloat16, device=device),
@@ -144,17 +127,18 @@ class WindowCache:
         """Start over with prompts k, v [B, T, Hk, D] (any strides) of which the
         first ``lengths`` [B] tokens count (default: all); ``pos`` becomes the
         lengths. Lengths outside 0..T are clamped and set the status word."""
-        self._check(k, (self.batch, k.shape[1] if k.dim() == 4 else -1, self.n_kv_head, self.head_dim), "k")
+        if self.native:
+            self._cache.fill(k, v, lengths)
+            return
+        if k.dim() != 4:
+            raise ValueError(f"k must be [B, T, Hk, D], got {list(k.shape)}")
+        t = k.shape[1]
+        self._check(k, (self.batch, t, self.n_kv_head, self.head_dim), "k")
         self._check(v, k.shape, "v")
         if lengths is not None:
             lengths = self._positions(lengths, "lengths")
-        t = k.shape[1]
         if t == 0:
             self.pos.zero_()
-            return
-        if self.native:
-            native.lib().kv_cache_fill(_rows(k), _rows(v), lengths, self.pos, *self._rows, *self._params,
-                                       self.window, self.sinks)
             return
         n = torch.full_like(self.pos, t) if lengths is None else lengths.clamp(0, t)
         s = torch.arange(self.slots, device=self.device)[None, :]
@@ -179,15 +163,13 @@ class WindowCache:
         """Keys and values [B, Hk, slots, D] in slot order, 0 where no token is:
         the cache's dtype, or fp32 for 4 bits."""
         if self.native:
-            return tuple(native.lib().kv_cache_read(self.pos, *self._rows, *self._params, self.window, self.sinks,
-                                                    self.head_dim))
+            return tuple(self._cache.read())
         seen = torch.arange(self.slots, device=self.device)[None, :] < self.pos[:, None]
         rows = (x if self.bits == 16 else dequantize_rows(*x) for x in self._rows)
         return tuple(torch.where(seen[:, None, :, None], x, torch.zeros((), dtype=x.dtype, device=x.device))
                      for x in rows)
 
     # ----------------------------------------------------------------- step
-    @torch.no_grad()
     def step(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, pos: Optional[torch.Tensor] = None,
              return_stored: bool = False):
         """One token per sequence: q [B, H, D], k and v [B, Hk, D] (any strides;
@@ -198,28 +180,21 @@ class WindowCache:
         nothing, result 0). By default the cache's own ``pos``, which advances.
         ``return_stored`` also returns what the stored key and value stand for
         (fp32 [B, Hk, D], 0 for idle sequences)."""
-        if q.dim() != 3 or q.shape[1] % self.n_kv_head or not q.shape[1]:
-            raise ValueError(f"q must be [B, H, D] with H a multiple of {self.n_kv_head}, got {list(q.shape)}")
-        self._check(q, (self.batch, q.shape[1], self.head_dim), "q")
-        self._check(k, (self.batch, self.n_kv_head, self.head_dim), "k")
-        self._check(v, k.shape, "v")
-        at = self._positions(self.pos if pos is None else pos, "pos")
+        at = self.pos if pos is None else pos
         if self.native:
-            heads = q.shape[1]
-            if heads not in self._work:
-                splits, floats, units = native.lib().kv_cache_plan(self.batch, self.n_kv_head, heads, self.head_dim,
-                                                                   self.slots, self.bits == 4)
-                self._work[heads] = (splits, torch.empty(floats, dtype=torch.float32, device=self.device),
-                                     torch.zeros(units, dtype=torch.int32, device=self.device))
-            splits, partial, arrived = self._work[heads]
-            result = native.lib().kv_cache_step(_rows(q), _rows(k), _rows(v), at, *self._rows, *self._params, partial,
-                                                arrived, self.window, self.sinks, splits, return_stored)
+            result = self._cache.step(q, k, v, at, return_stored)
         else:
-            result = self._plain_step(q, k, v, at, return_stored)
+            if q.dim() != 3 or q.shape[1] % self.n_kv_head or not q.shape[1]:
+                raise ValueError(f"q must be [B, H, D] with H a multiple of {self.n_kv_head}, got {list(q.shape)}")
+            self._check(q, (self.batch, q.shape[1], self.head_dim), "q")
+            self._check(k, (self.batch, self.n_kv_head, self.head_dim), "k")
+            self._check(v, k.shape, "v")
+            result = self._plain_step(q, k, v, self._positions(at, "pos"), return_stored)
         if pos is None:
             self.pos += (self.pos >= 0)
         return tuple(result) if return_stored else result[0]
 
+    @torch.no_grad()
     def _plain_step(self, q, k, v, pos, return_stored):
         on = (pos >= 0)[:, None, None]
         which = torch.arange(self.slots, device=self.device)[None, :] == self.slot_of(pos)[:, None]

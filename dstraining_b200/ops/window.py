@@ -52,59 +52,9 @@ def _check(window: int, sinks: int) -> None:
         raise ValueError(f"sinks must not be negative, got {sinks}")
 
 
-def _addressable(x: torch.Tensor) -> torch.Tensor:
-    """x itself if the tensor maps can address it, else a contiguous copy."""
-    ok = x.stride(3) == 1 and x.data_ptr() % 16 == 0
-    ok = ok and all(x.shape[i] == 1 or (x.stride(i) > 0 and x.stride(i) % 8 == 0) for i in range(3))
-    return x if ok else x.clone(memory_format=torch.contiguous_format)
-
-
 def _split(qkv: torch.Tensor, n_head: int, head_dim: int):
     b, t, _ = qkv.shape
     return qkv.view(b, t, n_head, 3, head_dim).unbind(dim=3)
-
-
-class _WindowFn(torch.autograd.Function):
-    """Separate q, k, v."""
-
-    @staticmethod
-    def forward(ctx, q, k, v, window, sinks):
-        q, k, v = _addressable(q), _addressable(k), _addressable(v)
-        out, lse = native.lib().window_attn_fwd(q, k, v, window, sinks)
-        ctx.save_for_backward(q, k, v, out, lse)
-        ctx.meta = (window, sinks)
-        return out
-
-    @staticmethod
-    def backward(ctx, dout):
-        q, k, v, out, lse = ctx.saved_tensors
-        dq, dk, dv = (torch.empty(x.shape, dtype=x.dtype, device=x.device) for x in (q, k, v))
-        native.lib().window_attn_bwd(_addressable(dout.contiguous()), q, k, v, out, lse, dq, dk, dv, *ctx.meta)
-        return dq, dk, dv, None, None
-
-
-class _WindowFusedFn(torch.autograd.Function):
-    """q, k, v interleaved head by head in one buffer, and their gradients likewise."""
-
-    @staticmethod
-    def forward(ctx, qkv, n_head, head_dim, window, sinks):
-        qkv = qkv.contiguous()
-        if qkv.data_ptr() % 16:
-            qkv = qkv.clone()
-        out, lse = native.lib().window_attn_fwd(*_split(qkv, n_head, head_dim), window, sinks)
-        ctx.save_for_backward(qkv, out, lse)
-        ctx.meta = (n_head, head_dim, window, sinks)
-        return out.view(*qkv.shape[:2], n_head * head_dim)
-
-    @staticmethod
-    def backward(ctx, dout):
-        qkv, out, lse = ctx.saved_tensors
-        n_head, head_dim, window, sinks = ctx.meta
-        dqkv = torch.empty_like(qkv)
-        native.lib().window_attn_bwd(
-            _addressable(dout.contiguous().view(out.shape)), *_split(qkv, n_head, head_dim), out, lse,
-            *_split(dqkv, n_head, head_dim), window, sinks)
-        return dqkv, None, None, None, None
 
 
 def window_attention(qkv: torch.Tensor, n_head: int, head_dim: int, window: int, sinks: int = 0) -> torch.Tensor:
@@ -115,7 +65,7 @@ def window_attention(qkv: torch.Tensor, n_head: int, head_dim: int, window: int,
         raise ValueError(f"qkv must be [B, T, {3 * n_head * head_dim}], got {tuple(qkv.shape)}")
     b, t, _ = qkv.shape
     if native.active(qkv) and b and t:
-        return _WindowFusedFn.apply(qkv, n_head, head_dim, window, sinks)
+        return native.lib().window_attention(qkv, n_head, head_dim, window, sinks)
     return core_window_attention(*_split(qkv.contiguous(), n_head, head_dim), window, sinks).reshape(b, t, n_head * head_dim)
 
 
@@ -129,5 +79,5 @@ def window_attention_qkv(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, wind
     if not k.shape[2] or q.shape[2] % k.shape[2]:
         raise ValueError(f"{q.shape[2]} query heads cannot share {k.shape[2]} key heads evenly")
     if native.active(q, k, v) and q.numel():
-        return _WindowFn.apply(q, k, v, window, sinks)
+        return native.lib().window_attention_qkv(q, k, v, window, sinks)
     return core_window_attention(q, k, v, window, sinks)

@@ -254,8 +254,9 @@ def test_refusals():
         with pytest.raises(RuntimeError, match="head_dim"):
             window_attention_qkv(*[_rand(1, 8, 2, d, seed=i) for i in range(3)], 4)
     lib = native.lib()
-    with pytest.raises(RuntimeError, match="strides"):
-        lib.window_attn_fwd(x[0].expand(2, 8, 2, 64), x[1].expand(2, 8, 2, 64), x[2].expand(2, 8, 2, 64), 4, 0)
-    out, lse = lib.window_attn_fwd(*x, 4, 0)
-    with pytest.raises(RuntimeError, match="lse"):
-        lib.window_attn_bwd(x[0], *x, out, lse[:, :1], *[torch.empty_like(t) for t in x], 4, 0)
+    with pytest.raises(RuntimeError, match="must be a CUDA bf16"):
+        lib.window_attention_qkv(x[0].float(), x[1], x[2], 4, 0)
+    with pytest.raises(RuntimeError, match="agree"):
+        lib.window_attention_qkv(x[0], x[1][:, :7], x[2][:, :7], 4, 0)
+    with pytest.raises(RuntimeError, match="window >= 1"):
+        lib.window_attention(_rand(1, 8, 3 * 128, seed=0), 2, 64, 0, 0)
