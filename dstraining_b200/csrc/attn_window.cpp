@@ -74,8 +74,8 @@ Shape shape_of(int64_t B, int64_t T, int64_t H, int64_t Hk, int64_t D, int64_t w
 template <int DP>
 void run_fwd(const Operand& q, const Operand& k, const Operand& v, __nv_bfloat16* out, float* lse, int64_t B,
              const Shape& s) {
-  const int Hk = s.H / s.G, rows = kFwdKeys;
-  launch_fwd<DP>(map_of(q, B, s.T, s.H, s.D, 128), map_of(k, B, s.T, Hk, s.D, rows), map_of(v, B, s.T, Hk, s.D, rows), out,
+  const int Hk = s.H / s.G;
+  launch_fwd<DP>(map_of(q, B, s.T, s.H, s.D, 128), map_of(k, B, s.T, Hk, s.D, 64), map_of(v, B, s.T, Hk, s.D, 64), out,
                  lse, B, s, at::cuda::getCurrentCUDAStream());
   C10_CUDA_KERNEL_LAUNCH_CHECK();
 }

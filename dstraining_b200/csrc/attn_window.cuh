@@ -42,7 +42,6 @@ namespace attn_window {
 
 constexpr int kRowAtom = 128 * 128;  // 128 rows x 64 channels, 128B-swizzled
 constexpr int kBlkAtom = 64 * 128;   // 64 rows x 64 channels
-constexpr int kFwdKeys = 128;        // keys of a forward block
 
 struct Shape {
   int T, Tp;    // tokens; rounded up to a multiple of 128 (rows of lse and di)
@@ -242,11 +241,6 @@ struct KeyBlocks {
     n = sink_blocks + q_last / BN - first + 1;
   }
   __device__ __forceinline__ int at(int j) const { return j < sink_blocks ? j : first + j - sink_blocks; }
-  // Whether some row of the tile sees some of the N keys from k0.
-  template <int N>
-  static __device__ __forceinline__ bool seen(const Shape& s, int q0, int k0) {
-    return k0 <= min(q0 + 127, s.T - 1) && (k0 + N > q0 - s.W + 1 || k0 < s.S);
-  }
   // Whether some row of the tile misses some of the N keys from k0.
   template <int N>
   static __device__ __forceinline__ bool partial(const Shape& s, int q0, int k0) {
