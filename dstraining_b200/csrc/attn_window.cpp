@@ -72,11 +72,11 @@ Shape shape_of(int64_t B, int64_t T, int64_t H, int64_t Hk, int64_t D, int64_t w
 }
 
 template <int DP>
-void run_fwd(const Operand& q, const Operand& k, const Operand& v, __nv_bfloat16* out, float* lse, int64_t B,
+void run_fwd(const Operand& q, const Operand& k, const Operand& v, const Operand& out, float* lse, int64_t B,
              const Shape& s) {
   const int Hk = s.H / s.G;
-  launch_fwd<DP>(map_of(q, B, s.T, s.H, s.D, 128), map_of(k, B, s.T, Hk, s.D, 64), map_of(v, B, s.T, Hk, s.D, 64), out,
-                 lse, B, s, at::cuda::getCurrentCUDAStream());
+  launch_fwd<DP>(map_of(q, B, s.T, s.H, s.D, 128), map_of(k, B, s.T, Hk, s.D, 64), map_of(v, B, s.T, Hk, s.D, 64),
+                 map_of(out, B, s.T, s.H, s.D, 128), lse, B, s, at::cuda::getCurrentCUDAStream());
   C10_CUDA_KERNEL_LAUNCH_CHECK();
 }
 
@@ -109,10 +109,11 @@ void run_bwd(__nv_bfloat16* dout, const Operand& q, const Operand& k, const Oper
   }
   const CUtensorMap k64 = map_of(k, B, s.T, Hk, s.D, 64), v64 = map_of(v, B, s.T, Hk, s.D, 64);
   launch_dkdv<DP>(map_of(q, B, s.T, s.H, s.D, 64), map_of(go, B, s.T, s.H, s.D, 64), map_of(k, B, s.T, Hk, s.D, 128),
-                  map_of(v, B, s.T, Hk, s.D, 128), lse, di, dk, dv, B, sinks, s, st);
+                  map_of(v, B, s.T, Hk, s.D, 128), lse, di, map_of(dk, B, s.T, Hk, s.D, 128),
+                  map_of(dv, B, s.T, Hk, s.D, 128), B, sinks, s, st);
   C10_CUDA_KERNEL_LAUNCH_CHECK();
-  launch_dq<DP>(map_of(q, B, s.T, s.H, s.D, 128), map_of(go, B, s.T, s.H, s.D, 128), k64, v64, lse, di, dq, dk, dv, B,
-                sinks, s, st);
+  launch_dq<DP>(map_of(q, B, s.T, s.H, s.D, 128), map_of(go, B, s.T, s.H, s.D, 128), k64, v64, lse, di,
+                map_of(dq, B, s.T, s.H, s.D, 128), dk, dv, B, sinks, s, st);
   C10_CUDA_KERNEL_LAUNCH_CHECK();
 }
 
@@ -121,7 +122,7 @@ std::pair<at::Tensor, at::Tensor> forward(const Operand& q, const Operand& k, co
                                           const Shape& s, const at::TensorOptions& options) {
   at::Tensor out = at::empty({B, s.T, s.H, s.D}, options);
   at::Tensor lse = at::empty({B, s.H, s.Tp}, options.dtype(at::kFloat));
-  auto* o = static_cast<__nv_bfloat16*>(out.data_ptr());
+  const Operand o = operand(out);
   if (s.D <= 64)
     run_fwd<64>(q, k, v, o, lse.data_ptr<float>(), B, s);
   else

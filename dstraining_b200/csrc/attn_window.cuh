@@ -99,6 +99,19 @@ __device__ __forceinline__ void tma_load_4d(uint32_t el, void* smem_dst, const C
       : "memory");
 }
 
+// 4-D tiled store of a 128-row tile's 64-channel atom; rows and channels past the
+// tensor's end are clipped.
+__device__ __forceinline__ void tma_store_4d(uint32_t el, const CUtensorMap* map, const void* smem_src, int c, int t,
+                                             int h, int b) {
+  asm volatile(
+      "{\n\t.reg .pred pe;\n\t"
+      "setp.ne.b32 pe, %6, 0;\n\t"
+      "@pe cp.async.bulk.tensor.4d.global.shared::cta.bulk_group [%0, {%2, %3, %4, %5}], [%1];\n\t}" ::"l"(
+          reinterpret_cast<uint64_t>(map)),
+      "r"(smem_u32(smem_src)), "r"(c), "r"(t), "r"(h), "r"(b), "r"(el)
+      : "memory");
+}
+
 __device__ __forceinline__ void expect_tx(uint32_t el, uint64_t* bar, uint32_t bytes) {
   if (el) mbar_arrive_expect_tx(bar, bytes);
 }
@@ -181,18 +194,24 @@ __device__ __forceinline__ void tmem_put32(uint32_t taddr, const float* v) {
 
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
-// Columns [c0, c0 + 32) of a row to global memory as bf16, up to D.
-__device__ __forceinline__ void store_cols(__nv_bfloat16* row, int c0, int D, const float (&v)[32], float scale) {
+// Columns [c0, c0 + 32) of row r of a 128B-swizzled result tile, as bf16.
+__device__ __forceinline__ void stage_cols(uint8_t* tile, int r, int c0, const float (&v)[32], float scale) {
+  uint8_t* row = tile + (c0 >> 6) * kRowAtom + r * 128;
 #pragma unroll
-  for (int i = 0; i < 32; i += 8) {
-    if (c0 + i < D) {
-      uint4 pk;
-      uint32_t* w = reinterpret_cast<uint32_t*>(&pk);
+  for (int i = 0; i < 4; ++i) {
+    uint4 pk;
+    uint32_t* w = reinterpret_cast<uint32_t*>(&pk);
 #pragma unroll
-      for (int t = 0; t < 4; ++t) w[t] = pack_bf16(v[i + 2 * t] * scale, v[i + 2 * t + 1] * scale);
-      *reinterpret_cast<uint4*>(row + c0 + i) = pk;
-    }
+    for (int t = 0; t < 4; ++t) w[t] = pack_bf16(v[8 * i + 2 * t] * scale, v[8 * i + 2 * t + 1] * scale);
+    *reinterpret_cast<uint4*>(row + (((((c0 >> 3) & 7) + i) ^ (r & 7)) << 4)) = pk;
   }
+}
+
+// The whole warp: a staged tile of DP channels to rows t.. of (head, sequence).
+template <int DP>
+__device__ __forceinline__ void store_tile(uint32_t el, const CUtensorMap* map, const uint8_t* tile, int t, int h, int b) {
+#pragma unroll
+  for (int a = 0; a < DP / 64; ++a) tma_store_4d(el, map, tile + a * kRowAtom, a * 64, t, h, b);
 }
 
 // 16 columns of a row, scaled in place.
@@ -261,19 +280,19 @@ __device__ __forceinline__ void mask_keys(float (&v)[N], const Shape& s, int q, 
 
 // Launches (padded head size DP = 64 or 128), on `stream`.
 template <int DP>
-void launch_fwd(const CUtensorMap& q128, const CUtensorMap& k, const CUtensorMap& v, __nv_bfloat16* out, float* lse,
-                int64_t B, const Shape& s, cudaStream_t stream);
+void launch_fwd(const CUtensorMap& q128, const CUtensorMap& k64, const CUtensorMap& v64, const CUtensorMap& out128,
+                float* lse, int64_t B, const Shape& s, cudaStream_t stream);
 template <int DP>
 void launch_rowdot(const __nv_bfloat16* dout, const __nv_bfloat16* out, float* di, int64_t B, const Shape& s,
                    cudaStream_t stream);
 template <int DP>
 void launch_dkdv(const CUtensorMap& q64, const CUtensorMap& dout64, const CUtensorMap& k128, const CUtensorMap& v128,
-                 const float* lse, const float* di, const Operand& dk, const Operand& dv, int64_t B,
+                 const float* lse, const float* di, const CUtensorMap& dk128, const CUtensorMap& dv128, int64_t B,
                  const SinkChunks& sinks, const Shape& s, cudaStream_t stream);
 template <int DP>
 void launch_dq(const CUtensorMap& q128, const CUtensorMap& dout128, const CUtensorMap& k64, const CUtensorMap& v64,
-               const float* lse, const float* di, const Operand& dq, const Operand& dk, const Operand& dv, int64_t B,
-               const SinkChunks& sinks, const Shape& s, cudaStream_t stream);
+               const float* lse, const float* di, const CUtensorMap& dq128, const Operand& dk, const Operand& dv,
+               int64_t B, const SinkChunks& sinks, const Shape& s, cudaStream_t stream);
 
 // Dynamic shared memory above 48 KB has to be allowed once per kernel and device.
 template <auto kKernel>

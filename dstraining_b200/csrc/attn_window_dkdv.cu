@@ -32,8 +32,8 @@ template <int DP>
 __global__ void __launch_bounds__(DkdvCfg<DP>::kThreads, DkdvCfg<DP>::kCtas)
     dkdv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmDO,
                 const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
-                const float* __restrict__ lse, const float* __restrict__ di, const Operand dk, const Operand dv,
-                const SinkChunks sinks, const Shape s) {
+                const __grid_constant__ CUtensorMap tmDK, const __grid_constant__ CUtensorMap tmDV,
+                const float* __restrict__ lse, const float* __restrict__ di, const SinkChunks sinks, const Shape s) {
   using C = DkdvCfg<DP>;
   constexpr int NB = C::NB, NS = C::NS;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
@@ -71,7 +71,7 @@ __global__ void __launch_bounds__(DkdvCfg<DP>::kThreads, DkdvCfg<DP>::kCtas)
   const int nq = qb1 - qb0 + 1, n = nq * s.G;
   const int warp = __shfl_sync(0xffffffff, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
 
-  if (threadIdx.x == 0) {
+  if (threadIdx.x == 32) {
     mbar_init(kv_full, 1);
     for (int i = 0; i < NS; ++i) {
       mbar_init(&q_full[i], 1);
@@ -85,6 +85,34 @@ __global__ void __launch_bounds__(DkdvCfg<DP>::kThreads, DkdvCfg<DP>::kCtas)
     }
     fence_barrier_init();
   }
+  int loaded = 0;  // query blocks whose copies were started (warp 1)
+  auto load_q = [&](uint32_t el) {
+    const int st = loaded % NS, h = hk * s.G + loaded / nq, q0 = (qb0 + loaded % nq) * 64;
+    expect_tx(el, &q_full[st], 2 * C::kQ + 512);
+#pragma unroll
+    for (int a = 0; a < C::kAt; ++a) {
+      tma_load_4d(el, sQ + st * C::kQ + a * kBlkAtom, &tmQ, &q_full[st], a * 64, q0, h, b);
+      tma_load_4d(el, sDO + st * C::kQ + a * kBlkAtom, &tmDO, &q_full[st], a * 64, q0, h, b);
+    }
+    const int64_t row = (static_cast<int64_t>(b) * s.H + h) * s.Tp + q0;
+    if (el) {
+      bulk_load(sL + st * 64, lse + row, 256, &q_full[st]);
+      bulk_load(sDi + st * 64, di + row, 256, &q_full[st]);
+    }
+    __syncwarp();
+    ++loaded;
+  };
+  if (warp == 1) {  // the first copies travel while TMEM is allocated
+    __syncwarp();
+    const uint32_t el = elect_one();
+    expect_tx(el, kv_full, 2 * C::kKV);
+#pragma unroll
+    for (int a = 0; a < C::kAt; ++a) {
+      tma_load_4d(el, sK + a * kRowAtom, &tmK, kv_full, a * 64, k0, hk, b);
+      tma_load_4d(el, sV + a * kRowAtom, &tmV, kv_full, a * 64, k0, hk, b);
+    }
+    while (loaded < min(n, NS)) load_q(el);
+  }
   if (warp == 0) {
     __syncwarp();
     tmem_alloc(tmem_slot, C::kTmem);
@@ -93,36 +121,14 @@ __global__ void __launch_bounds__(DkdvCfg<DP>::kThreads, DkdvCfg<DP>::kCtas)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
+  bool done = warp < 2;  // this thread's part of the result is staged
   const uint32_t tmem = __shfl_sync(0xffffffff, *tmem_slot, 0);
   // pair i: S^T in columns 128 i.., dP^T in 128 i + 64..; then dV, dK
   const uint32_t tDV = tmem + 128 * NB, tDK = tDV + DP;
 
   if (warp == 1) {
     const uint32_t el = elect_one();
-    expect_tx(el, kv_full, 2 * C::kKV);
-#pragma unroll
-    for (int a = 0; a < C::kAt; ++a) {
-      tma_load_4d(el, sK + a * kRowAtom, &tmK, kv_full, a * 64, k0, hk, b);
-      tma_load_4d(el, sV + a * kRowAtom, &tmV, kv_full, a * 64, k0, hk, b);
-    }
-    int loaded = 0;
-    for (int h = hk * s.G, q = 0; loaded < n; ++loaded, ++q) {
-      if (q == nq) q = 0, ++h;
-      const int st = loaded % NS, q0 = (qb0 + q) * 64;
-      if (!warp_wait(&q_empty[st], ((loaded / NS) & 1) ^ 1, s.status, kTimeoutSmemEmpty)) break;
-      expect_tx(el, &q_full[st], 2 * C::kQ + 512);
-#pragma unroll
-      for (int a = 0; a < C::kAt; ++a) {
-        tma_load_4d(el, sQ + st * C::kQ + a * kBlkAtom, &tmQ, &q_full[st], a * 64, q0, h, b);
-        tma_load_4d(el, sDO + st * C::kQ + a * kBlkAtom, &tmDO, &q_full[st], a * 64, q0, h, b);
-      }
-      const int64_t row = (static_cast<int64_t>(b) * s.H + h) * s.Tp + q0;
-      if (el) {
-        bulk_load(sL + st * 64, lse + row, 256, &q_full[st]);
-        bulk_load(sDi + st * 64, di + row, 256, &q_full[st]);
-      }
-      __syncwarp();
-    }
+    while (loaded < n && warp_wait(&q_empty[loaded % NS], ((loaded / NS) & 1) ^ 1, s.status, kTimeoutSmemEmpty)) load_q(el);
     // no copy may land after the CTA is gone
     mbar_wait(kv_full, 0, s.status, kTimeoutTmaFull);
     for (int i = max(0, loaded - NS); i < loaded; ++i)
@@ -219,9 +225,8 @@ __global__ void __launch_bounds__(DkdvCfg<DP>::kThreads, DkdvCfg<DP>::kCtas)
       // 2 NB threads a row, each a share of the columns of dK and dV
       constexpr int kShare = DP / (2 * NB);
       const int c0 = group * kShare;
+      // sink rows of a cut block are sums of a chunk only: joined over the stored tile later
       const bool to_partial = cut && key < s.S;
-      __nv_bfloat16* krow = dk.p + b * dk.s.b + static_cast<int64_t>(key) * dk.s.t + hk * dk.s.h;
-      __nv_bfloat16* vrow = dv.p + b * dv.s.b + static_cast<int64_t>(key) * dv.s.t + hk * dv.s.h;
       float* part = cut ? sinks.partial +
                               ((((static_cast<int64_t>(b) * gridDim.y + hk) * sinks.blocks + kb) * (1 + sinks.chunks) + chunk) *
                                    2 * 128 + r) * DP
@@ -237,15 +242,24 @@ __global__ void __launch_bounds__(DkdvCfg<DP>::kThreads, DkdvCfg<DP>::kCtas)
             float4* dst = reinterpret_cast<float4*>(part + which * 128 * DP + c);
 #pragma unroll
             for (int j = 0; j < 8; ++j) dst[j] = make_float4(x[4 * j], x[4 * j + 1], x[4 * j + 2], x[4 * j + 3]);
-          } else if (chunk == 0 && key < s.T) {
-            store_cols(which ? vrow : krow, c, s.D, x, which ? 1.f : s.scale);
           }
+          if (chunk == 0) stage_cols(which ? sV : sK, r, c, x, which ? 1.f : s.scale);
         }
       }
+      fence_proxy_async_smem();
+      done = true;
     }
   }
   tc_fence_before();
-  __syncthreads();
+  if (__syncthreads_and(done) && warp == 1 && chunk == 0) {
+    const uint32_t el = elect_one();
+    store_tile<DP>(el, &tmDK, sK, k0, hk, b);
+    store_tile<DP>(el, &tmDV, sV, k0, hk, b);
+    if (el) {
+      bulk_commit();
+      bulk_wait_read<0>();
+    }
+  }
   if (warp == 0) {
     tc_fence_after();
     tmem_dealloc(tmem, C::kTmem);
@@ -289,20 +303,20 @@ void launch_rowdot(const __nv_bfloat16* dout, const __nv_bfloat16* out, float* d
 
 template <int DP>
 void launch_dkdv(const CUtensorMap& q64, const CUtensorMap& dout64, const CUtensorMap& k128, const CUtensorMap& v128,
-                 const float* lse, const float* di, const Operand& dk, const Operand& dv, int64_t B,
+                 const float* lse, const float* di, const CUtensorMap& dk128, const CUtensorMap& dv128, int64_t B,
                  const SinkChunks& sinks, const Shape& s, cudaStream_t stream) {
   using C = DkdvCfg<DP>;
   if (allow_smem<dkdv_kernel<DP>>(C::kSmem) != cudaSuccess) return;
   const dim3 grid(s.Tp / 128 + sinks.blocks * sinks.chunks, s.H / s.G, static_cast<unsigned>(B));
-  dkdv_kernel<DP><<<grid, C::kThreads, C::kSmem, stream>>>(q64, dout64, k128, v128, lse, di, dk, dv, sinks, s);
+  dkdv_kernel<DP><<<grid, C::kThreads, C::kSmem, stream>>>(q64, dout64, k128, v128, dk128, dv128, lse, di, sinks, s);
 }
 
 #define INSTANCES(DP)                                                                                                   \
   template void launch_rowdot<DP>(const __nv_bfloat16*, const __nv_bfloat16*, float*, int64_t, const Shape&,            \
                                   cudaStream_t);                                                                        \
   template void launch_dkdv<DP>(const CUtensorMap&, const CUtensorMap&, const CUtensorMap&, const CUtensorMap&,         \
-                                const float*, const float*, const Operand&, const Operand&, int64_t, const SinkChunks&, \
-                                const Shape&, cudaStream_t);
+                                const float*, const float*, const CUtensorMap&, const CUtensorMap&, int64_t,            \
+                                const SinkChunks&, const Shape&, cudaStream_t);
 INSTANCES(64)
 INSTANCES(128)
 

@@ -28,8 +28,8 @@ template <int DP>
 __global__ void __launch_bounds__(kThreads, 2)
     dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmDO,
               const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
-              const float* __restrict__ lse, const float* __restrict__ di, const Operand dq, const Operand dk,
-              const Operand dv, const SinkChunks sinks, const Shape s) {
+              const __grid_constant__ CUtensorMap tmDQ, const float* __restrict__ lse, const float* __restrict__ di,
+              const Operand dk, const Operand dv, const SinkChunks sinks, const Shape s) {
   using C = DqCfg<DP>;
   constexpr int NV = C::NV;
   extern __shared__ __align__(1024) uint8_t smem[];
@@ -75,6 +75,14 @@ __global__ void __launch_bounds__(kThreads, 2)
   const KeyBlocks<64> blocks(s, q0);
   const int n = blocks.n;
 
+  int ks = 0, vs = 0;  // copies started (warp 0)
+  auto load = [&](uint32_t el, const CUtensorMap* map, uint8_t* dst, uint64_t* bar, int j) {
+    expect_tx(el, bar, C::kKV);
+#pragma unroll
+    for (int a = 0; a < C::kAt; ++a) tma_load_4d(el, dst + a * kBlkAtom, map, bar, a * 64, blocks.at(j) * 64, hk, b);
+  };
+  auto load_k = [&](uint32_t el) { load(el, &tmK, sK + (ks % 2) * C::kKV, &k_full[ks % 2], ks), ++ks; };
+  auto load_v = [&](uint32_t el) { load(el, &tmV, sV + (vs % NV) * C::kKV, &v_full[vs % NV], vs), ++vs; };
   if (threadIdx.x == 0) {
     mbar_init(q_full, 1);
     for (int i = 0; i < 2; ++i) {
@@ -86,43 +94,39 @@ __global__ void __launch_bounds__(kThreads, 2)
     mbar_init(g_full, 1);
     fence_barrier_init();
   }
-  if (warp == 0) {
+  if (warp == 0) {  // the first copies travel while TMEM is allocated
     __syncwarp();
+    const uint32_t el = elect_one();
+    expect_tx(el, q_full, 2 * C::kQ);
+#pragma unroll
+    for (int a = 0; a < C::kAt; ++a) {
+      tma_load_4d(el, sDO + a * kRowAtom, &tmDO, q_full, a * 64, q0, h, b);
+      tma_load_4d(el, sQ + a * kRowAtom, &tmQ, q_full, a * 64, q0, h, b);
+    }
+    while (vs < min(n, NV)) load_v(el);
+    while (ks < min(n, 2)) load_k(el);
+  }
+  if (warp == 1) {
     tmem_alloc(tmem_slot, 256);
     tmem_relinquish();
   }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
+  bool done = warp == 0;  // this thread's part of the result is staged
   const uint32_t tmem = __shfl_sync(0xffffffff, *tmem_slot, 0);
   const uint32_t tDP = tmem + 64, tDQ = tmem + 128;  // S, and dS over it, from 0
 
   if (warp == 0) {
-    constexpr uint32_t id_s = idesc_bf16_f32(128, 64, false, false), id_g = idesc_bf16_f32(128, DP, false, true);
     const uint32_t el = elect_one();
-    auto load = [&](const CUtensorMap* map, uint8_t* dst, uint64_t* bar, int j) {
-      expect_tx(el, bar, C::kKV);
-#pragma unroll
-      for (int a = 0; a < C::kAt; ++a) tma_load_4d(el, dst + a * kBlkAtom, map, bar, a * 64, blocks.at(j) * 64, hk, b);
-    };
-    int ks = 0, vs = 0;  // copies started
-    expect_tx(el, q_full, 2 * C::kQ);
-#pragma unroll
-    for (int a = 0; a < C::kAt; ++a) {
-      tma_load_4d(el, sQ + a * kRowAtom, &tmQ, q_full, a * 64, q0, h, b);
-      tma_load_4d(el, sDO + a * kRowAtom, &tmDO, q_full, a * 64, q0, h, b);
-    }
-    auto load_k = [&]() { load(&tmK, sK + (ks % 2) * C::kKV, &k_full[ks % 2], ks), ++ks; };
-    auto load_v = [&]() { load(&tmV, sV + (vs % NV) * C::kKV, &v_full[vs % NV], vs), ++vs; };
-    while (vs < min(n, NV)) load_v();
-    while (ks < min(n, 2)) load_k();
+    constexpr uint32_t id_s = idesc_bf16_f32(128, 64, false, false), id_g = idesc_bf16_f32(128, DP, false, true);
     bool ok = warp_wait(q_full, 0, s.status, kTimeoutTmaFull);
     for (int j = 0; j <= n && ok; ++j) {
       if (j > 0) {
         const int g = j - 1;
         // dP_g has been read by its product
         ok = warp_wait(s_full, g & 1, s.status, kTimeoutTmemFull);
-        if (ok && vs < n) load_v();
+        if (ok && vs < n) load_v(el);
         ok = ok && warp_wait(p_full, g & 1, s.status, kTimeoutTmemFull);
         if (!ok) break;
         tc_fence_after();
@@ -138,7 +142,7 @@ __global__ void __launch_bounds__(kThreads, 2)
         product<DP>(el, tDP, sDO, sV + (j % NV) * C::kKV, kBlkAtom, id_s);
         if (j > 0) {  // dS over S, and K of the block before
           ok = warp_wait(g_full, (j - 1) & 1, s.status, kTimeoutTmemFull);
-          if (ok && ks < n) load_k();
+          if (ok && ks < n) load_k(el);
         }
         ok = ok && warp_wait(&k_full[j % 2], (j / 2) & 1, s.status, kTimeoutTmaFull);
         if (!ok) break;
@@ -181,19 +185,27 @@ __global__ void __launch_bounds__(kThreads, 2)
     }
     if (__all_sync(0xffffffff, ok && mbar_wait(g_full, (n - 1) & 1, s.status, kTimeoutTmemFull))) {
       tc_fence_after();
-      __nv_bfloat16* qrow = dq.p + b * dq.s.b + static_cast<int64_t>(q) * dq.s.t + h * dq.s.h;
 #pragma unroll
       for (int ch = 0; ch < DP / 64; ++ch) {
         const int c = half * (DP / 2) + ch * 32;
         float x[32];
         tmem_ld32_sync(tDQ + c + lane_off, x);
-        if (q < s.T) store_cols(qrow, c, s.D, x, s.scale);
+        stage_cols(sQ, r, c, x, s.scale);
       }
+      fence_proxy_async_smem();
+      done = true;
     }
   }
   tc_fence_before();
-  __syncthreads();
-  if (warp == 0) {
+  if (__syncthreads_and(done) && warp == 0) {
+    const uint32_t el = elect_one();
+    store_tile<DP>(el, &tmDQ, sQ, q0, h, b);
+    if (el) {
+      bulk_commit();
+      bulk_wait_read<0>();
+    }
+  }
+  if (warp == 1) {
     tc_fence_after();
     tmem_dealloc(tmem, 256);
   }
@@ -201,16 +213,17 @@ __global__ void __launch_bounds__(kThreads, 2)
 
 template <int DP>
 void launch_dq(const CUtensorMap& q128, const CUtensorMap& dout128, const CUtensorMap& k64, const CUtensorMap& v64,
-               const float* lse, const float* di, const Operand& dq, const Operand& dk, const Operand& dv, int64_t B,
-               const SinkChunks& sinks, const Shape& s, cudaStream_t stream) {
+               const float* lse, const float* di, const CUtensorMap& dq128, const Operand& dk, const Operand& dv,
+               int64_t B, const SinkChunks& sinks, const Shape& s, cudaStream_t stream) {
   if (allow_smem<dq_kernel<DP>>(DqCfg<DP>::kSmem) != cudaSuccess) return;
   const dim3 grid(s.Tp / 128 + sinks.blocks, s.H, static_cast<unsigned>(B));
-  dq_kernel<DP><<<grid, kThreads, DqCfg<DP>::kSmem, stream>>>(q128, dout128, k64, v64, lse, di, dq, dk, dv, sinks, s);
+  dq_kernel<DP><<<grid, kThreads, DqCfg<DP>::kSmem, stream>>>(q128, dout128, k64, v64, dq128, lse, di, dk, dv, sinks, s);
 }
 
 #define INSTANCE(DP)                                                                                                  \
   template void launch_dq<DP>(const CUtensorMap&, const CUtensorMap&, const CUtensorMap&, const CUtensorMap&,         \
-                              const float*, const float*, const Operand&, const Operand&, const Operand&, int64_t,    \
+                              const float*, const float*, const CUtensorMap&, const Operand&, const Operand&,         \
+                              int64_t,                                                                                \
                               const SinkChunks&, const Shape&, cudaStream_t);
 INSTANCE(64)
 INSTANCE(128)

@@ -28,8 +28,8 @@ struct FwdCfg {
 template <int DP>
 __global__ void __launch_bounds__(kThreads, 2)
     fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
-               const __grid_constant__ CUtensorMap tmV, __nv_bfloat16* __restrict__ out, float* __restrict__ lse,
-               const Shape s) {
+               const __grid_constant__ CUtensorMap tmV, const __grid_constant__ CUtensorMap tmO,
+               float* __restrict__ lse, const Shape s) {
   using C = FwdCfg<DP>;
   constexpr int NS = C::NS;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
@@ -53,6 +53,14 @@ __global__ void __launch_bounds__(kThreads, 2)
   const KeyBlocks<64> blocks(s, q0);
   const int n = blocks.n;
 
+  int ks = 0, vs = 0;  // copies started (warp 0)
+  auto load = [&](uint32_t el, const CUtensorMap* map, uint8_t* dst, uint64_t* bar, int j) {
+    expect_tx(el, bar, C::kKV);
+#pragma unroll
+    for (int a = 0; a < C::kAt; ++a) tma_load_4d(el, dst + a * kBlkAtom, map, bar, a * 64, blocks.at(j) * 64, hk, b);
+  };
+  auto load_k = [&](uint32_t el) { load(el, &tmK, sK + (ks % NS) * C::kKV, &k_full[ks % NS], ks), ++ks; };
+  auto load_v = [&](uint32_t el) { load(el, &tmV, sV + (vs % NS) * C::kKV, &v_full[vs % NS], vs), ++vs; };
   if (threadIdx.x == 0) {
     mbar_init(q_full, 1);
     for (int i = 0; i < NS; ++i) {
@@ -66,27 +74,30 @@ __global__ void __launch_bounds__(kThreads, 2)
     mbar_init(o_full, 1);
     fence_barrier_init();
   }
-  if (warp == 0) {
+  if (warp == 0) {  // the first copies travel while TMEM is allocated
     __syncwarp();
+    const uint32_t el = elect_one();
+    expect_tx(el, q_full, C::kQ);
+#pragma unroll
+    for (int a = 0; a < C::kAt; ++a) tma_load_4d(el, sQ + a * kRowAtom, &tmQ, q_full, a * 64, q0, h, b);
+    while (ks < min(n, NS)) {
+      load_k(el);
+      load_v(el);
+    }
+  }
+  if (warp == 1) {
     tmem_alloc(tmem_slot, 256);
     tmem_relinquish();
   }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
+  bool done = warp == 0;  // this thread's part of the result is staged
   const uint32_t tmem = __shfl_sync(0xffffffff, *tmem_slot, 0);
 
   if (warp == 0) {
     const uint32_t el = elect_one();
     constexpr uint32_t id_s = idesc_bf16_f32(128, 64, false, false), id_o = idesc_bf16_f32(128, DP, false, true);
-    auto load = [&](const CUtensorMap* map, uint8_t* dst, uint64_t* bar, int j) {
-      expect_tx(el, bar, C::kKV);
-#pragma unroll
-      for (int a = 0; a < C::kAt; ++a) tma_load_4d(el, dst + a * kBlkAtom, map, bar, a * 64, blocks.at(j) * 64, hk, b);
-    };
-    int ks = 0, vs = 0;  // copies started
-    auto load_k = [&]() { load(&tmK, sK + (ks % NS) * C::kKV, &k_full[ks % NS], ks), ++ks; };
-    auto load_v = [&]() { load(&tmV, sV + (vs % NS) * C::kKV, &v_full[vs % NS], vs), ++vs; };
     auto issue_s = [&](int j) -> bool {  // S = Q K_j^T
       if (!warp_wait(&k_full[j % NS], (j / NS) & 1, s.status, kTimeoutTmaFull)) return false;
       tc_fence_after();
@@ -94,19 +105,12 @@ __global__ void __launch_bounds__(kThreads, 2)
       mma_commit(el, &s_full[j & 1]);
       return true;
     };
-    expect_tx(el, q_full, C::kQ);
-#pragma unroll
-    for (int a = 0; a < C::kAt; ++a) tma_load_4d(el, sQ + a * kRowAtom, &tmQ, q_full, a * 64, q0, h, b);
-    while (ks < min(n, NS)) {
-      load_k();
-      load_v();
-    }
     bool ok = warp_wait(q_full, 0, s.status, kTimeoutTmaFull) && issue_s(0) && (n == 1 || issue_s(1));
     for (int j = 0; j < n && ok; ++j) {
       ok = warp_wait(&v_full[j % NS], (j / NS) & 1, s.status, kTimeoutTmaFull) &&
            warp_wait(&p_full[j & 1], (j >> 1) & 1, s.status, kTimeoutTmemFull);
       if (!ok) break;
-      if (ks < n) load_k();  // into K_j's stage: its scores are long done
+      if (ks < n) load_k(el);  // into K_j's stage: its scores are long done
       tc_fence_after();
       const uint32_t v = desc_lo(sV + (j % NS) * C::kKV, kBlkAtom);
 #pragma unroll
@@ -116,7 +120,7 @@ __global__ void __launch_bounds__(kThreads, 2)
       mma_commit(el, o_full);
       if (j + 2 < n) {  // V_j, and the buffer of S_j and P_j, are free once this is done
         ok = warp_wait(o_full, j & 1, s.status, kTimeoutTmemFull);
-        if (ok) load_v();
+        if (ok) load_v(el);
         ok = ok && issue_s(j + 2);
       }
     }
@@ -189,36 +193,44 @@ __global__ void __launch_bounds__(kThreads, 2)
     if (__all_sync(0xffffffff, ok && mbar_wait(o_full, (n - 1) & 1, s.status, kTimeoutTmemFull))) {
       tc_fence_after();
       const float inv = 1.f / l;
-      __nv_bfloat16* row = out + ((static_cast<int64_t>(b) * s.T + q) * s.H + h) * s.D;
 #pragma unroll
       for (int ch = 0; ch < DP / 64; ++ch) {
         float o[32];
         tmem_ld32_sync(tmem + C::kO + half * (DP / 2) + ch * 32 + lane_off, o);
-        if (q < s.T) store_cols(row, half * (DP / 2) + ch * 32, s.D, o, inv);
+        stage_cols(sQ, r, half * (DP / 2) + ch * 32, o, inv);
       }
+      fence_proxy_async_smem();
+      done = true;
       // rows past the end: +inf, so that their probabilities are 0 in backward
       if (half == 0)
         lse[(static_cast<int64_t>(b) * s.H + h) * s.Tp + q] = q < s.T ? m_ref + log2f(l) : INFINITY;
     }
   }
   tc_fence_before();
-  __syncthreads();
-  if (warp == 0) {
+  if (__syncthreads_and(done) && warp == 0) {
+    const uint32_t el = elect_one();
+    store_tile<DP>(el, &tmO, sQ, q0, h, b);
+    if (el) {
+      bulk_commit();
+      bulk_wait_read<0>();
+    }
+  }
+  if (warp == 1) {
     tc_fence_after();
     tmem_dealloc(tmem, 256);
   }
 }
 
 template <int DP>
-void launch_fwd(const CUtensorMap& q128, const CUtensorMap& k, const CUtensorMap& v, __nv_bfloat16* out, float* lse,
-                int64_t B, const Shape& s, cudaStream_t stream) {
+void launch_fwd(const CUtensorMap& q128, const CUtensorMap& k64, const CUtensorMap& v64, const CUtensorMap& out128,
+                float* lse, int64_t B, const Shape& s, cudaStream_t stream) {
   if (allow_smem<fwd_kernel<DP>>(FwdCfg<DP>::kSmem) != cudaSuccess) return;
-  fwd_kernel<DP><<<dim3(s.Tp / 128, s.H, static_cast<unsigned>(B)), kThreads, FwdCfg<DP>::kSmem, stream>>>(q128, k, v, out,
-                                                                                                       lse, s);
+  fwd_kernel<DP><<<dim3(s.Tp / 128, s.H, static_cast<unsigned>(B)), kThreads, FwdCfg<DP>::kSmem, stream>>>(
+      q128, k64, v64, out128, lse, s);
 }
-template void launch_fwd<64>(const CUtensorMap&, const CUtensorMap&, const CUtensorMap&, __nv_bfloat16*, float*, int64_t,
-                             const Shape&, cudaStream_t);
-template void launch_fwd<128>(const CUtensorMap&, const CUtensorMap&, const CUtensorMap&, __nv_bfloat16*, float*, int64_t,
-                              const Shape&, cudaStream_t);
+template void launch_fwd<64>(const CUtensorMap&, const CUtensorMap&, const CUtensorMap&, const CUtensorMap&, float*,
+                             int64_t, const Shape&, cudaStream_t);
+template void launch_fwd<128>(const CUtensorMap&, const CUtensorMap&, const CUtensorMap&, const CUtensorMap&, float*,
+                              int64_t, const Shape&, cudaStream_t);
 }  // namespace attn_window
 }  // namespace dst
