@@ -279,14 +279,24 @@ __device__ __forceinline__ void split2(float x, float y, uint32_t& hi, uint32_t&
   lo = pack2(x - __uint_as_float(hi << 16), y - __uint_as_float(hi & 0xffff0000u));
 }
 
-template <int DP, int BITS>
+// What the 8 query rows of the mma are.
+enum Rows {
+  kBf16Heads,      // bf16 cache: a head each
+  kPackedHeads,    // 4 bits: a head each; every thread handles all groups of its keys
+  kPackedGroups,   // 4 bits, few heads per key head: (head, group of 32 channels) each, so that a
+                   // thread applies the steps and least values of its own group only
+};
+
+template <int DP, int ROWS>
 struct StepCfg {
+  static constexpr bool kPacked = ROWS != kBf16Heads;
   static constexpr int NG = DP / 32;
-  static constexpr int kRowBytes = BITS == 16 ? DP * 2 : DP / 2;
-  static constexpr int kParamBytes = BITS == 16 ? 0 : NG * 4;
+  static constexpr int kHeads = ROWS == kPackedGroups ? kRows / NG : kRows;  // per CTA
+  static constexpr int kRowBytes = kPacked ? DP / 2 : DP * 2;
+  static constexpr int kParamBytes = kPacked ? NG * 4 : 0;
   // keys per stage of a warp's ring
-  static constexpr int KT = BITS == 16 ? (DP == 64 ? 32 : 16) : (DP == 64 ? 64 : 32);
-  static constexpr int kStages = BITS == 16 ? 3 : 2;
+  static constexpr int KT = kPacked ? (DP == 64 ? 64 : 32) : (DP == 64 ? 32 : 16);
+  static constexpr int kStages = kPacked ? 2 : 3;
   static constexpr int kOperand = KT * kRowBytes;  // keys or values of a stage
   static constexpr int kStage = 2 * kOperand + 2 * KT * kParamBytes;
   static constexpr int kRingBytes = kWarps * kStages * kStage;
@@ -294,7 +304,7 @@ struct StepCfg {
   static constexpr int kNew = 2 * 16 * (kRowBytes + kParamBytes);
   static constexpr int kJoin = kWarps * kRows * (DP + 2) * 4;  // over the ring at the end
   static constexpr int kSmem = (kRingBytes > kJoin ? kRingBytes : kJoin) + kNew + kWarps * kStages * 8 + 16 + 1024;
-  static constexpr int kCtas = BITS == 16 ? 2 : (DP == 64 ? 4 : 3);  // per SM
+  static constexpr int kCtas = kPacked ? (DP == 64 ? 4 : 3) : 2;  // per SM
 };
 
 struct StepArgs {
@@ -315,13 +325,26 @@ struct StepArgs {
 
 // The warp's running result for the 8 query rows: thread (n = lane / 4, t =
 // lane % 4) holds for row n the output channels of columns 2t, 2t + 1 of each
-// 8-column tile, and the parts of l and of the constant terms that its keys add.
-template <int DP, int BITS>
+// 8-column tile. The codes enter as 128 + code, and a value has its group's least
+// value: both make a term that is the same for all channels of a group,
+// sum over keys of p low - 128 p step.
+template <int DP, int ROWS>
 struct State {
-  static constexpr int NG = DP / 32;
-  float m, l;
+  float m, l;          // l: of this thread's keys
   float o[DP / 8][4];  // [tile]: 0, 1 high parts, 2, 3 low parts
-  float c[BITS == 4 ? NG : 1];  // sum of p (low - 128 step)
+  float c[4];          // packed heads: that term for group 2t, 2t + 1 (high, low parts);
+                       // packed groups: -128 sum p step of this row's group
+  float low;           // packed groups: sum p low, of this thread's keys
+};
+
+// The query rows as A operands, and their sums over groups.
+template <int DP, int ROWS>
+struct Query {
+  uint32_t a[DP / 16][2];
+  // packed heads: -128 sum q per group, and the sums as three bf16 parts to be
+  // multiplied with the least values of a key; packed groups: the row's own sum
+  float off[ROWS == kPackedHeads ? DP / 32 : 1];
+  uint32_t sum[2];
 };
 
 // One 16-byte chunk `c` of row `r` of a 128B-swizzled tile of 64 channels.
@@ -329,29 +352,34 @@ __device__ __forceinline__ const uint4* swz(const uint8_t* tile, int r, int c) {
   return reinterpret_cast<const uint4*>(tile + r * 128 + ((c ^ (r & 7)) << 4));
 }
 
+__device__ __forceinline__ uint32_t code_pair(uint32_t w, int i) {  // 128 + code, twice
+  return ((w >> (4 * i)) & 0x000f000fu) | 0x43004300u;
+}
+
 // NS subtiles of 16 keys each: keys and values at `sk`, `sv` (and their
-// parameters), `rows_in_tile` rows per swizzled tile; bit i of `valid` says
-// whether key i takes part.
-template <int DP, int BITS, int NS>
-__device__ __forceinline__ void attend(State<DP, BITS>& st, const uint32_t (&qa)[DP / 16][2], const float* qsum,
-                                       const uint8_t* sk, const uint8_t* sv, const uint32_t* pk, const uint32_t* pv,
-                                       int tile_rows, uint32_t valid, float scale_log2) {
+// parameters), `tile_rows` rows per swizzled tile; bit i of `valid` says whether
+// key i takes part.
+template <int DP, int ROWS, int NS>
+__device__ __forceinline__ void attend(State<DP, ROWS>& st, const Query<DP, ROWS>& q, const uint8_t* sk,
+                                       const uint8_t* sv, const uint32_t* pk, const uint32_t* pv, int tile_rows,
+                                       uint32_t valid, float scale_log2) {
   constexpr int NG = DP / 32;
   const int lane = threadIdx.x & 31, n = lane >> 2, t = lane & 3;
+  const int group = n & (NG - 1);  // of this row, where rows are (head, group)
   constexpr uint32_t kAll = NS == 2 ? 0xffffffffu : 0xffffu;
   float s[2 * NS][2];  // scores of columns 2t, 2t + 1 of each 8 keys, row n
 #pragma unroll
   for (int i = 0; i < 2 * NS; ++i) {
     const int r = i * 8 + n;
-    if (BITS == 16) {
+    if constexpr (ROWS == kBf16Heads) {
       float acc[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int a = 0; a < DP / 64; ++a) {
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
           const uint4 w = *swz(sk + a * tile_rows * 128, r, 2 * t + c);
-          mma16816(acc, qa[a * 4 + c * 2][0], 0u, qa[a * 4 + c * 2][1], 0u, w.x, w.y);
-          mma16816(acc, qa[a * 4 + c * 2 + 1][0], 0u, qa[a * 4 + c * 2 + 1][1], 0u, w.z, w.w);
+          mma16816(acc, q.a[a * 4 + c * 2][0], 0u, q.a[a * 4 + c * 2][1], 0u, w.x, w.y);
+          mma16816(acc, q.a[a * 4 + c * 2 + 1][0], 0u, q.a[a * 4 + c * 2 + 1][1], 0u, w.z, w.w);
         }
       }
       s[i][0] = acc[0];
@@ -359,27 +387,52 @@ __device__ __forceinline__ void attend(State<DP, BITS>& st, const uint32_t (&qa)
     } else {
       uint32_t w[NG];
       const uint8_t* p = sk + r * (DP / 2) + t * (DP / 8);
-      if (NG == 2) {
+      if constexpr (NG == 2) {
         const uint2 u = *reinterpret_cast<const uint2*>(p);
         w[0] = u.x, w[1] = u.y;
       } else {
         const uint4 u = *reinterpret_cast<const uint4*>(p);
-        w[0] = u.x, w[1] = u.y, w[NG - 2] = u.z, w[NG - 1] = u.w;
+        w[0] = u.x, w[1] = u.y, w[2] = u.z, w[3] = u.w;
       }
-      s[i][0] = s[i][1] = 0.f;
+      const uint32_t* par = pk + (i * 8 + 2 * t) * NG;  // of the keys of columns 2t, 2t + 1
+      if constexpr (ROWS == kPackedGroups) {
+        float acc[4] = {q.off[0] * -128.f, q.off[0] * -128.f, 0.f, 0.f};
 #pragma unroll
-      for (int g = 0; g < NG; ++g) {
-        float acc[4] = {0.f, 0.f, 0.f, 0.f};
-        uint32_t b[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) b[j] = ((w[g] >> (4 * j)) & 0x000f000fu) | 0x43004300u;
-        mma16816(acc, qa[2 * g][0], 0u, qa[2 * g][1], 0u, b[0], b[1]);
-        mma16816(acc, qa[2 * g + 1][0], 0u, qa[2 * g + 1][1], 0u, b[2], b[3]);
+        for (int g = 0; g < NG; ++g) {  // rows of other groups hold zeros there
+          mma16816(acc, q.a[2 * g][0], 0u, q.a[2 * g][1], 0u, code_pair(w[g], 0), code_pair(w[g], 1));
+          mma16816(acc, q.a[2 * g + 1][0], 0u, q.a[2 * g + 1][1], 0u, code_pair(w[g], 2), code_pair(w[g], 3));
+        }
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          const uint32_t par = pk[(i * 8 + 2 * t + e) * NG + g];
-          const float step = param_step(par);
-          s[i][e] += fmaf(step, acc[e], fmaf(-128.f, step, param_low(par)) * qsum[g]);
+          const uint32_t x = par[e * NG + group];
+          float v = fmaf(param_step(x), acc[e], param_low(x) * q.off[0]);
+          v += __shfl_xor_sync(0xffffffff, v, 4);  // the groups of a head lie in neighbouring rows
+          if (NG == 4) v += __shfl_xor_sync(0xffffffff, v, 8);
+          s[i][e] = v;
+        }
+      } else {
+        // least values times query sums: k-slots (2t, 2t + 1) and (2t + 8, 2t + 9)
+        float base[4] = {0.f, 0.f, 0.f, 0.f};
+        const uint2 lw = *reinterpret_cast<const uint2*>(pk + r * NG + (NG == 4 ? 2 * (t & 1) : 0));
+        const uint32_t lows = __byte_perm(lw.x, lw.y, 0x7632);
+        mma16816(base, q.sum[0], 0u, q.sum[1], 0u, lows, NG == 4 && t < 2 ? lows : 0u);
+        s[i][0] = base[0];
+        s[i][1] = base[1];
+        uint32_t step[2][NG];
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+#pragma unroll
+          for (int g = 0; g < NG; g += 2) {
+            const uint2 x = *reinterpret_cast<const uint2*>(par + e * NG + g);
+            step[e][g] = x.x, step[e][g + 1] = x.y;
+          }
+#pragma unroll
+        for (int g = 0; g < NG; ++g) {
+          float acc[4] = {q.off[g], q.off[g], 0.f, 0.f};
+          mma16816(acc, q.a[2 * g][0], 0u, q.a[2 * g][1], 0u, code_pair(w[g], 0), code_pair(w[g], 1));
+          mma16816(acc, q.a[2 * g + 1][0], 0u, q.a[2 * g + 1][1], 0u, code_pair(w[g], 2), code_pair(w[g], 3));
+          s[i][0] = fmaf(param_step(step[0][g]), acc[0], s[i][0]);
+          s[i][1] = fmaf(param_step(step[1][g]), acc[1], s[i][1]);
         }
       }
     }
@@ -407,9 +460,10 @@ __device__ __forceinline__ void attend(State<DP, BITS>& st, const uint32_t (&qa)
     for (int i = 0; i < DP / 8; ++i)
 #pragma unroll
       for (int j = 0; j < 4; ++j) st.o[i][j] *= c;
-    if (BITS == 4) {
+    if constexpr (ROWS != kBf16Heads) {
 #pragma unroll
-      for (int g = 0; g < NG; ++g) st.c[g] *= c;
+      for (int j = 0; j < 4; ++j) st.c[j] *= c;
+      st.low *= c;
     }
   }
   const float m_use = st.m == -INFINITY ? 0.f : st.m;
@@ -424,20 +478,21 @@ __device__ __forceinline__ void attend(State<DP, BITS>& st, const uint32_t (&qa)
   for (int u = 0; u < NS; ++u) {
     const int r0 = u * 16 + 2 * t;  // this thread's keys: r0, r0 + 1, r0 + 8, r0 + 9
     const uint32_t in = valid >> r0;
-    if (BITS == 16) {
+    // what lies in a masked row must not meet its zero probability
+    const bool on[4] = {(in & 1u) != 0, (in & 2u) != 0, (in & 0x100u) != 0, (in & 0x200u) != 0};
+    const float p[4] = {s[2 * u][0], s[2 * u][1], s[2 * u + 1][0], s[2 * u + 1][1]};
+    if constexpr (ROWS == kBf16Heads) {
       uint32_t a0, a1, a2, a3;
-      split2(s[2 * u][0], s[2 * u][1], a0, a1);
-      split2(s[2 * u + 1][0], s[2 * u + 1][1], a2, a3);
+      split2(p[0], p[1], a0, a1);
+      split2(p[2], p[3], a2, a3);
 #pragma unroll
       for (int a = 0; a < DP / 64; ++a) {
         const uint8_t* tile = sv + a * tile_rows * 128;
         uint4 x[4] = {*swz(tile, r0, n), *swz(tile, r0 + 1, n), *swz(tile, r0 + 8, n), *swz(tile, r0 + 9, n)};
-        if (valid != kAll) {  // what lies in a masked row must not meet its zero probability
-          const uint4 z = make_uint4(0, 0, 0, 0);
-          if (!(in & 1u)) x[0] = z;
-          if (!(in & 2u)) x[1] = z;
-          if (!(in & 0x100u)) x[2] = z;
-          if (!(in & 0x200u)) x[3] = z;
+        if (valid != kAll) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            if (!on[j]) x[j] = make_uint4(0, 0, 0, 0);
         }
         const uint32_t* w[4] = {&x[0].x, &x[1].x, &x[2].x, &x[3].x};
 #pragma unroll
@@ -452,50 +507,85 @@ __device__ __forceinline__ void attend(State<DP, BITS>& st, const uint32_t (&qa)
       uint32_t w[4][NG / 2];
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const uint8_t* p = sv + (r0 + (j & 1) + (j >> 1) * 8) * (DP / 2) + n * (DP / 16);
-        if (NG == 2) {
-          w[j][0] = *reinterpret_cast<const uint32_t*>(p);
+        const uint8_t* x = sv + (r0 + (j & 1) + (j >> 1) * 8) * (DP / 2) + n * (DP / 16);
+        if constexpr (NG == 2) {
+          w[j][0] = *reinterpret_cast<const uint32_t*>(x);
         } else {
-          const uint2 x = *reinterpret_cast<const uint2*>(p);
-          w[j][0] = x.x, w[j][NG / 2 - 1] = x.y;
+          const uint2 y = *reinterpret_cast<const uint2*>(x);
+          w[j][0] = y.x, w[j][1] = y.y;
         }
       }
-#pragma unroll
-      for (int g = 0; g < NG; ++g) {
+      constexpr uint32_t kMinus128 = 0xc300c300u;
+      if constexpr (ROWS == kPackedGroups) {
         float x[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          uint32_t par = pv[(r0 + (j & 1) + (j >> 1) * 8) * NG + g];
-          if (valid != kAll && !((in >> ((j & 1) + (j >> 1) * 8)) & 1u)) par = 0u;
-          const float p = s[2 * u + (j >> 1)][j & 1], step = param_step(par);
-          x[j] = p * step;
-          st.c[g] = fmaf(p, fmaf(-128.f, step, param_low(par)), st.c[g]);
+          uint32_t par = pv[(r0 + (j & 1) + (j >> 1) * 8) * NG + group];
+          if (valid != kAll && !on[j]) par = 0u;
+          x[j] = p[j] * param_step(par);
+          st.low = fmaf(p[j], param_low(par), st.low);
         }
         uint32_t a0, a1, a2, a3;
         split2(x[0], x[1], a0, a1);
         split2(x[2], x[3], a2, a3);
-        const uint32_t sel = (g & 1) ? 0x7632 : 0x5410;
-        const uint32_t lo = __byte_perm(w[0][g >> 1], w[1][g >> 1], sel);
-        const uint32_t hi = __byte_perm(w[2][g >> 1], w[3][g >> 1], sel);
+        mma16816(st.c, a0, a1, a2, a3, kMinus128, kMinus128);
+#pragma unroll
+        for (int g = 0; g < NG; ++g) {
+          const uint32_t lo = __byte_perm(w[0][g >> 1], w[1][g >> 1], (g & 1) ? 0x7632 : 0x5410);
+          const uint32_t hi = __byte_perm(w[2][g >> 1], w[3][g >> 1], (g & 1) ? 0x7632 : 0x5410);
+#pragma unroll
+          for (int j = 0; j < 4; ++j)  // meaningful in the rows of group g
+            mma16816(st.o[g * 4 + j], a0, a1, a2, a3, code_pair(lo, j), code_pair(hi, j));
+        }
+      } else {
+        uint32_t par[4][NG];
 #pragma unroll
         for (int j = 0; j < 4; ++j)
-          mma16816(st.o[g * 4 + j], a0, a1, a2, a3, ((lo >> (4 * j)) & 0x000f000fu) | 0x43004300u,
-                   ((hi >> (4 * j)) & 0x000f000fu) | 0x43004300u);
+#pragma unroll
+          for (int g = 0; g < NG; g += 2) {
+            const uint2 x = *reinterpret_cast<const uint2*>(pv + (r0 + (j & 1) + (j >> 1) * 8) * NG + g);
+            par[j][g] = x.x, par[j][g + 1] = x.y;
+          }
+        // least values: columns n of the constant terms are groups n % NG
+        uint32_t a0, a1, a2, a3, lw[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          lw[j] = pv[(r0 + (j & 1) + (j >> 1) * 8) * NG + group];
+          if (valid != kAll && !on[j]) {
+            lw[j] = 0u;
+#pragma unroll
+            for (int g = 0; g < NG; ++g) par[j][g] = 0u;
+          }
+        }
+        split2(p[0], p[1], a0, a1);
+        split2(p[2], p[3], a2, a3);
+        mma16816(st.c, a0, a1, a2, a3, __byte_perm(lw[0], lw[1], 0x7632), __byte_perm(lw[2], lw[3], 0x7632));
+#pragma unroll
+        for (int g = 0; g < NG; ++g) {
+          split2(p[0] * param_step(par[0][g]), p[1] * param_step(par[1][g]), a0, a1);
+          split2(p[2] * param_step(par[2][g]), p[3] * param_step(par[3][g]), a2, a3);
+          const uint32_t col = group == g ? kMinus128 : 0u;
+          mma16816(st.c, a0, a1, a2, a3, col, col);
+          const uint32_t lo = __byte_perm(w[0][g >> 1], w[1][g >> 1], (g & 1) ? 0x7632 : 0x5410);
+          const uint32_t hi = __byte_perm(w[2][g >> 1], w[3][g >> 1], (g & 1) ? 0x7632 : 0x5410);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) mma16816(st.o[g * 4 + j], a0, a1, a2, a3, code_pair(lo, j), code_pair(hi, j));
+        }
       }
     }
   }
 }
 
 // Output channel of tile `tile`, column `n`.
-template <int DP, int BITS>
+template <int DP, int ROWS>
 __device__ __forceinline__ int channel_of(int tile, int n) {
-  return BITS == 16 ? (tile >> 3) * 64 + n * 8 + (tile & 7) : (tile >> 2) * 32 + n * 4 + (tile & 3);
+  return ROWS == kBf16Heads ? (tile >> 3) * 64 + n * 8 + (tile & 7) : (tile >> 2) * 32 + n * 4 + (tile & 3);
 }
 
-template <int DP, int BITS>
-__global__ void __launch_bounds__(kThreads, StepCfg<DP, BITS>::kCtas)
+template <int DP, int ROWS>
+__global__ void __launch_bounds__(kThreads, StepCfg<DP, ROWS>::kCtas)
     step_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const StepArgs a) {
-  using C = StepCfg<DP, BITS>;
+  using C = StepCfg<DP, ROWS>;
   constexpr int NG = C::NG, KT = C::KT, ST = C::kStages;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -506,8 +596,8 @@ __global__ void __launch_bounds__(kThreads, StepCfg<DP, BITS>::kCtas)
   const int split = blockIdx.x, b = blockIdx.z;
   const int hk = blockIdx.y / a.chunks, chunk = blockIdx.y % a.chunks;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, n = lane >> 2, t = lane & 3;
-  const int heads = min(kRows, a.G - chunk * kRows);  // query heads of this CTA
-  const int h0 = hk * a.G + chunk * kRows;
+  const int heads = min(C::kHeads, a.G - chunk * C::kHeads);  // query heads of this CTA
+  const int h0 = hk * a.G + chunk * C::kHeads;
   const int64_t p = a.pos[b];
   if (p < 0) {  // an idle sequence: nothing to see, nothing to store
     if (split == 0) {
@@ -546,7 +636,7 @@ __global__ void __launch_bounds__(kThreads, StepCfg<DP, BITS>::kCtas)
     const int64_t row = base + first + (warp + i * kWarps) * KT;
     uint8_t* dst = ring + stage * C::kStage;
     mbar_arrive_expect_tx(&full[stage], C::kStage);
-    if (BITS == 16) {
+    if (!C::kPacked) {
 #pragma unroll
       for (int c = 0; c < DP / 64; ++c) {
         tma_load_2d(dst + c * KT * 128, &tmK, &full[stage], c * 64, static_cast<int>(row));
@@ -567,45 +657,61 @@ __global__ void __launch_bounds__(kThreads, StepCfg<DP, BITS>::kCtas)
 
   // Query rows as the A operand. Channels of k-step kk that thread t holds: for
   // bf16 keys (kk/4)*64 + t*16 + (kk%4)*4 + 0..3, for packed keys (kk/2)*32 +
-  // t*8 + (kk%2)*4 + 0..3.
-  uint32_t qa[DP / 16][2];
-  float qsum[NG];
+  // t*8 + (kk%2)*4 + 0..3. Where rows are (head, group), a row's other groups are 0.
+  const int row_head = ROWS == kPackedGroups ? n / NG : n, row_group = n & (NG - 1);
+  Query<DP, ROWS> q;
   {
-    const __nv_bfloat16* qrow = a.q + b * a.q_b + (h0 + n) * a.q_h;
+    const __nv_bfloat16* qrow = a.q + b * a.q_b + (h0 + row_head) * a.q_h;
+    float sum[NG];
+#pragma unroll
+    for (int g = 0; g < NG; ++g) sum[g] = 0.f;
 #pragma unroll
     for (int kk = 0; kk < DP / 16; ++kk) {
-      const int c = BITS == 16 ? (kk >> 2) * 64 + t * 16 + (kk & 3) * 4 : (kk >> 1) * 32 + t * 8 + (kk & 1) * 4;
-      const uint2 w = (n < heads && c < a.D) ? *reinterpret_cast<const uint2*>(qrow + c) : make_uint2(0u, 0u);
-      qa[kk][0] = w.x;
-      qa[kk][1] = w.y;
+      const int c = C::kPacked ? (kk >> 1) * 32 + t * 8 + (kk & 1) * 4 : (kk >> 2) * 64 + t * 16 + (kk & 3) * 4;
+      const bool on = row_head < heads && c < a.D && (ROWS != kPackedGroups || (kk >> 1) == row_group);
+      const uint2 w = on ? *reinterpret_cast<const uint2*>(qrow + c) : make_uint2(0u, 0u);
+      q.a[kk][0] = w.x;
+      q.a[kk][1] = w.y;
+      if (C::kPacked)
+        sum[kk >> 1] += (__uint_as_float(w.x << 16) + __uint_as_float(w.x & 0xffff0000u)) +
+                        (__uint_as_float(w.y << 16) + __uint_as_float(w.y & 0xffff0000u));
     }
+    if (C::kPacked) {
 #pragma unroll
-    for (int g = 0; g < NG; ++g) {
-      float x = 0.f;
-      if (BITS == 4) {
-#pragma unroll
-        for (int e = 0; e < 2; ++e)
-#pragma unroll
-          for (int w = 0; w < 2; ++w)
-            x += __uint_as_float(qa[2 * g + e][w] << 16) + __uint_as_float(qa[2 * g + e][w] & 0xffff0000u);
-        x += __shfl_xor_sync(0xffffffff, x, 1);
-        x += __shfl_xor_sync(0xffffffff, x, 2);
+      for (int g = 0; g < NG; ++g) {
+        sum[g] += __shfl_xor_sync(0xffffffff, sum[g], 1);
+        sum[g] += __shfl_xor_sync(0xffffffff, sum[g], 2);
       }
-      qsum[g] = x;
+      if constexpr (ROWS == kPackedGroups) {
+        q.off[0] = 0.f;
+#pragma unroll
+        for (int g = 0; g < NG; ++g) q.off[0] += sum[g];  // zero but for the row's own group
+      } else if constexpr (ROWS == kPackedHeads) {
+        // three bf16 parts of each sum; thread t holds part t / 2 of groups 2 (t % 2), + 1
+        // and, for t < 2, the third part (two groups: part t)
+        const int pair = NG == 4 ? 2 * (t & 1) : 0, part = NG == 4 ? t >> 1 : t;
+        const float s0 = pair ? sum[NG - 2] : sum[0], s1 = pair ? sum[NG - 1] : sum[1];
+        uint32_t hi, mid, lo, rest;
+        split2(s0, s1, hi, mid);
+        const float r0 = s0 - __uint_as_float(hi << 16), r1 = s1 - __uint_as_float(hi & 0xffff0000u);
+        split2(r0 - __uint_as_float(mid << 16), r1 - __uint_as_float(mid & 0xffff0000u), lo, rest);
+        q.sum[0] = part == 0 ? hi : part == 1 ? mid : (NG == 2 && part == 2) ? lo : 0u;
+        q.sum[1] = NG == 4 && t < 2 ? lo : 0u;
+#pragma unroll
+        for (int g = 0; g < NG; ++g) q.off[g] = -128.f * sum[g];
+      }
     }
   }
 
-  State<DP, BITS> st;
+  State<DP, ROWS> st;
   st.m = -INFINITY;
-  st.l = 0.f;
+  st.l = st.low = 0.f;
 #pragma unroll
   for (int i = 0; i < DP / 8; ++i)
 #pragma unroll
     for (int j = 0; j < 4; ++j) st.o[i][j] = 0.f;
-  if (BITS == 4) {
 #pragma unroll
-    for (int g = 0; g < NG; ++g) st.c[g] = 0.f;
-  }
+  for (int j = 0; j < 4; ++j) st.c[j] = 0.f;
 
   // The new token: its row into the cache (once) and, laid out as a tile of one
   // key, into this warp's result.
@@ -622,26 +728,26 @@ __global__ void __launch_bounds__(kThreads, StepCfg<DP, BITS>::kCtas)
     uint32_t* params = reinterpret_cast<uint32_t*>(fresh + 32 * C::kRowBytes) + (value ? 16 * NG : 0);
     float f[8];
     unpack8(u, f);
-    if (BITS == 16) {
+    if (!C::kPacked) {
       if (on) {
         *reinterpret_cast<uint4*>(tile + (i >> 3) * 16 * 128 + ((i & 7) << 4)) = u;  // row 0: chunks in order
         if (chunk == 0) *reinterpret_cast<uint4*>(s.rows + row * C::kRowBytes + i * 16) = u;
       }
     } else {
-      const Quant8 q = quantize8(f);
-      values8(q, f);
+      const Quant8 code = quantize8(f);
+      values8(code, f);
       if (on) {
         uint8_t* dst = s.rows + row * C::kRowBytes;
         if (value) {
-          put_value8<DP>(tile, i, q.code);
-          if (chunk == 0) put_value8<DP>(dst, i, q.code);
+          put_value8<DP>(tile, i, code.code);
+          if (chunk == 0) put_value8<DP>(dst, i, code.code);
         } else {
-          put_key8<DP>(tile, i, q.code);
-          if (chunk == 0) put_key8<DP>(dst, i, q.code);
+          put_key8<DP>(tile, i, code.code);
+          if (chunk == 0) put_key8<DP>(dst, i, code.code);
         }
         if ((i & 3) == 0) {
-          params[i >> 2] = q.param;
-          if (chunk == 0) s.params[row * NG + (i >> 2)] = q.param;
+          params[i >> 2] = code.param;
+          if (chunk == 0) s.params[row * NG + (i >> 2)] = code.param;
         }
       }
     }
@@ -649,7 +755,7 @@ __global__ void __launch_bounds__(kThreads, StepCfg<DP, BITS>::kCtas)
       store8f((value ? a.stored_v : a.stored_k) + bh * a.D + i * 8, f);
     __syncwarp();
     const uint32_t* fp = reinterpret_cast<const uint32_t*>(fresh + 32 * C::kRowBytes);
-    attend<DP, BITS, 1>(st, qa, qsum, fresh, fresh + 16 * C::kRowBytes, fp, fp + 16 * NG, 16, 1u, a.scale_log2);
+    attend<DP, ROWS, 1>(st, q, fresh, fresh + 16 * C::kRowBytes, fp, fp + 16 * NG, 16, 1u, a.scale_log2);
   }
 
   bool ok = true;
@@ -670,8 +776,8 @@ __global__ void __launch_bounds__(kThreads, StepCfg<DP, BITS>::kCtas)
       uint32_t valid = last - r >= 16 * NS ? kAll : (1u << (last - r)) - 1u;
       if (fresh_slot >= r && fresh_slot < r + 16 * NS) valid &= ~(1u << (fresh_slot - r));
       const int off = u * 16 * NS;
-      attend<DP, BITS, NS>(st, qa, qsum, src + off * (BITS == 16 ? 128 : C::kRowBytes),
-                           src + C::kOperand + off * (BITS == 16 ? 128 : C::kRowBytes), pk + off * NG, pv + off * NG,
+      attend<DP, ROWS, NS>(st, q, src + off * (C::kPacked ? C::kRowBytes : 128),
+                           src + C::kOperand + off * (C::kPacked ? C::kRowBytes : 128), pk + off * NG, pv + off * NG,
                            KT, valid, a.scale_log2);
     }
     __syncwarp();
@@ -684,24 +790,31 @@ __global__ void __launch_bounds__(kThreads, StepCfg<DP, BITS>::kCtas)
   // the keys of a row were spread over 4 lanes
   st.l += __shfl_xor_sync(0xffffffff, st.l, 1);
   st.l += __shfl_xor_sync(0xffffffff, st.l, 2);
-  if (BITS == 4) {
+  float add[NG];  // what all channels of a group get
 #pragma unroll
-    for (int g = 0; g < NG; ++g) {
-      st.c[g] += __shfl_xor_sync(0xffffffff, st.c[g], 1);
-      st.c[g] += __shfl_xor_sync(0xffffffff, st.c[g], 2);
-    }
+  for (int g = 0; g < NG; ++g) add[g] = 0.f;
+  if constexpr (ROWS == kPackedHeads) {
+    const float c0 = st.c[0] + st.c[2], c1 = st.c[1] + st.c[3];
+#pragma unroll
+    for (int g = 0; g < NG; ++g) add[g] = __shfl_sync(0xffffffff, (g & 1) ? c1 : c0, (lane & 28) + (g >> 1));
+  } else if constexpr (ROWS == kPackedGroups) {
+    st.low += __shfl_xor_sync(0xffffffff, st.low, 1);
+    st.low += __shfl_xor_sync(0xffffffff, st.low, 2);
+#pragma unroll
+    for (int g = 0; g < NG; ++g) add[g] = st.low + st.c[0] + st.c[2];
   }
   __syncthreads();  // every ring has been read
   float* join = reinterpret_cast<float*>(smem);  // [warp][row][DP + 2]: output, m, l
-  if (n < heads) {
-    float* row = join + (warp * kRows + n) * (DP + 2);
+  if (row_head < heads) {
+    float* row = join + (warp * kRows + row_head) * (DP + 2);
 #pragma unroll
     for (int i = 0; i < DP / 8; ++i) {
-      const float c = BITS == 4 ? st.c[i >> 2] : 0.f;
-      row[channel_of<DP, BITS>(i, 2 * t)] = st.o[i][0] + st.o[i][2] + c;
-      row[channel_of<DP, BITS>(i, 2 * t + 1)] = st.o[i][1] + st.o[i][3] + c;
+      if (ROWS == kPackedGroups && (i >> 2) != row_group) continue;  // another row's channels
+      const float c = C::kPacked ? add[i >> 2] : 0.f;
+      row[channel_of<DP, ROWS>(i, 2 * t)] = st.o[i][0] + st.o[i][2] + c;
+      row[channel_of<DP, ROWS>(i, 2 * t + 1)] = st.o[i][1] + st.o[i][3] + c;
     }
-    if (t == 0) {
+    if (t == 0 && (ROWS != kPackedGroups || row_group == 0)) {
       row[DP] = st.m;
       row[DP + 1] = st.l;
     }
@@ -807,7 +920,7 @@ class KVCache {
       if constexpr (bits_c() == 16) {
         const uint64_t n = static_cast<uint64_t>(B_) * Hk_ * alloc;
         for (int i = 0; i < 2; ++i)
-          map_[i] = make_tmap_bf16(rows_[i].data_ptr(), dp(), n, dp(), 64, StepCfg<dp(), 16>::KT);
+          map_[i] = make_tmap_bf16(rows_[i].data_ptr(), dp(), n, dp(), 64, StepCfg<dp(), kBf16Heads>::KT);
       }
     });
   }
@@ -864,7 +977,9 @@ class KVCache {
                                bool return_stored) {
     TORCH_CHECK_VALUE(q_.dim() == 3 && q_.size(1) >= 1 && q_.size(1) % Hk_ == 0, "q must be [B, H, D] with H a multiple of ",
                       std::to_string(Hk_), ", got ", sizes_text(q_.sizes()));
-    const int64_t H = q_.size(1), G = H / Hk_, chunks = (G + kRows - 1) / kRows;
+    const int64_t H = q_.size(1), G = H / Hk_;
+    const Rows rows = rows_for(G);
+    const int64_t per = rows == kPackedGroups ? kRows / (DP_ / 32) : kRows, chunks = (G + per - 1) / per;
     check_rows(q_, {B_, H, D_}, "q");
     check_rows(k_, {B_, Hk_, D_}, "k");
     check_rows(v_, {B_, Hk_, D_}, "v");
@@ -872,7 +987,7 @@ class KVCache {
     TORCH_CHECK_VALUE(Hk_ * chunks <= 65535, "kv cache: too many query heads");
     c10::cuda::CUDAGuard guard(pos_.device());
     const at::Tensor q = as_rows(q_), k = as_rows(k_), v = as_rows(v_);
-    const Work& work = work_for(chunks);
+    const Work& work = work_for(chunks, rows);
     at::Tensor out = at::empty({B_, H, D_}, q.options());
     std::vector<at::Tensor> result = {out};
     StepArgs a;
@@ -897,9 +1012,9 @@ class KVCache {
     a.scale_log2 = static_cast<float>(1.4426950408889634 / std::sqrt(static_cast<double>(D_)));
     a.status = status_ptr();
     const dim3 grid(static_cast<unsigned>(work.splits), static_cast<unsigned>(Hk_ * chunks), static_cast<unsigned>(B_));
-    dispatch([&](auto dp, auto bits) {
-      using C = StepCfg<dp(), bits()>;
-      auto kernel = step_kernel<dp(), bits()>;
+    dispatch_step(rows, [&](auto dp, auto rows_c) {
+      using C = StepCfg<dp(), static_cast<int>(rows_c())>;
+      auto kernel = step_kernel<dp(), static_cast<int>(rows_c())>;
       static bool configured[64] = {false};
       const int dev = pos_.device().index();
       if (!configured[dev])
@@ -930,15 +1045,32 @@ class KVCache {
     if (DP_ == 128 && bits_ == 4) f(integral_constant<int, 128>(), integral_constant<int, 4>());
   }
 
+  // 4 bits: rows of (head, group) as long as a key head's query heads fit in one CTA.
+  Rows rows_for(int64_t G) const {
+    if (bits_ == 16) return kBf16Heads;
+    return G <= kRows / (DP_ / 32) ? kPackedGroups : kPackedHeads;
+  }
+
+  template <typename F>
+  void dispatch_step(Rows rows, F&& f) const {
+    using std::integral_constant;
+    auto with = [&](auto dp) {
+      if (rows == kBf16Heads) f(dp, integral_constant<int, kBf16Heads>());
+      if (rows == kPackedHeads) f(dp, integral_constant<int, kPackedHeads>());
+      if (rows == kPackedGroups) f(dp, integral_constant<int, kPackedGroups>());
+    };
+    DP_ == 64 ? with(integral_constant<int, 64>()) : with(integral_constant<int, 128>());
+  }
+
   // How many CTAs share the slots of one (sequence, key head): enough to fill the
   // GPU, each with at least one tile per warp.
-  const Work& work_for(int64_t chunks) {
+  const Work& work_for(int64_t chunks, Rows rows) {
     auto it = work_.find(chunks);
     if (it != work_.end()) return it->second;
     const int64_t units = B_ * Hk_ * chunks;
     int64_t splits = 1;
-    dispatch([&](auto dp, auto bits) {
-      using C = StepCfg<dp(), bits()>;
+    dispatch_step(rows, [&](auto dp, auto rows_c) {
+      using C = StepCfg<dp(), static_cast<int>(rows_c())>;
       const int64_t most = (slots_ + kWarps * C::KT - 1) / (kWarps * C::KT);
       splits = std::min(most, std::max<int64_t>(1, (C::kCtas * num_sms() + units - 1) / units));
     });
