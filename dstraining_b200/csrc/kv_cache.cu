@@ -268,6 +268,21 @@ __device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
+__device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, float c0,
+                                         float c1, float c2, float c3) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c0), "f"(c1), "f"(c2), "f"(c3));
+}
+
+// 8 x 8 b16 matrix, a row per 4 lanes, transposed.
+__device__ __forceinline__ uint32_t transpose8(uint32_t x) {
+  uint32_t y;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+
 __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
   __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
   return *reinterpret_cast<uint32_t*>(&h);
@@ -304,7 +319,8 @@ struct StepCfg {
   static constexpr int kNew = 2 * 16 * (kRowBytes + kParamBytes);
   static constexpr int kJoin = kWarps * kRows * (DP + 2) * 4;  // over the ring at the end
   static constexpr int kSmem = (kRingBytes > kJoin ? kRingBytes : kJoin) + kNew + kWarps * kStages * 8 + 16 + 1024;
-  static constexpr int kCtas = kPacked ? (DP == 64 ? 4 : 3) : 2;  // per SM
+  static constexpr int kCtas = !kPacked ? 2 : ROWS == kPackedGroups ? 4 : DP == 64 ? 4 : 3;  // per SM
+  static constexpr int kSub = ROWS == kPackedHeads ? 1 : KT % 32 == 0 ? 2 : 1;  // subtiles of 16 keys at a time
 };
 
 struct StepArgs {
@@ -325,25 +341,33 @@ struct StepArgs {
 
 // The warp's running result for the 8 query rows: thread (n = lane / 4, t =
 // lane % 4) holds for row n the output channels of columns 2t, 2t + 1 of each
-// 8-column tile. The codes enter as 128 + code, and a value has its group's least
-// value: both make a term that is the same for all channels of a group,
-// sum over keys of p low - 128 p step.
+// 8-column tile.
+//
+// Packed rows: the scores are computed transposed (a row of the mma is a key, so
+// all 16 rows are used and the codes of a key go in as they come), so a thread's
+// m and l are those of the query rows 2t, 2t + 1, over its keys n, n + 8. The codes
+// enter as 128 + code, and a value has its group's least value: both make a term
+// that is the same for all channels of a group, sum over keys of p low - 128 p step.
 template <int DP, int ROWS>
 struct State {
-  float m, l;          // l: of this thread's keys
-  float o[DP / 8][4];  // [tile]: 0, 1 high parts, 2, 3 low parts
-  float c[4];          // packed heads: that term for group 2t, 2t + 1 (high, low parts);
-                       // packed groups: -128 sum p step of this row's group
-  float low;           // packed groups: sum p low, of this thread's keys
+  static constexpr int NG = DP / 32;
+  // packed groups: columns 2t, 2t + 1 are groups of one head, and the output is of the
+  // row's own group
+  static constexpr int kHeads = ROWS == kPackedHeads ? 2 : 1;
+  static constexpr int kTiles = ROWS == kPackedGroups ? 4 : DP / 8;
+  float m[kHeads], l[kHeads];
+  float o[kTiles][4];  // [tile]: 0, 1 high parts, 2, 3 low parts of the probabilities
+  float c[4];          // -128 sum p step: packed heads: of groups 2t, 2t + 1; packed groups: of the row's
+  float low[ROWS == kPackedHeads ? NG : 1][2];  // sum p low of (group,) query row 2t, 2t + 1
 };
 
-// The query rows as A operands, and their sums over groups.
+// The query rows as mma operands. Packed: also -128 times their sums over groups
+// for the query rows 2t, 2t + 1, and those sums to be multiplied with the least
+// values of a key (packed heads: as three bf16 parts).
 template <int DP, int ROWS>
 struct Query {
   uint32_t a[DP / 16][2];
-  // packed heads: -128 sum q per group, and the sums as three bf16 parts to be
-  // multiplied with the least values of a key; packed groups: the row's own sum
-  float off[ROWS == kPackedHeads ? DP / 32 : 1];
+  float off[ROWS == kPackedHeads ? DP / 32 : 1][2];
   uint32_t sum[2];
 };
 
@@ -352,90 +376,40 @@ __device__ __forceinline__ const uint4* swz(const uint8_t* tile, int r, int c) {
   return reinterpret_cast<const uint4*>(tile + r * 128 + ((c ^ (r & 7)) << 4));
 }
 
-__device__ __forceinline__ uint32_t code_pair(uint32_t w, int i) {  // 128 + code, twice
-  return ((w >> (4 * i)) & 0x000f000fu) | 0x43004300u;
+// As in the prompt's kernel a row keeps its reference maximum until a tile exceeds
+// it by 8 (in log2); then the sums of that row are rescaled by this factor.
+__device__ __forceinline__ float move_max(float& m, float& l, float mx) {
+  if (!(mx > m + 8.f)) return 1.f;
+  const float c = exp2f(m - mx);
+  m = mx;
+  l *= c;
+  return c;
 }
 
-// NS subtiles of 16 keys each: keys and values at `sk`, `sv` (and their
-// parameters), `tile_rows` rows per swizzled tile; bit i of `valid` says whether
-// key i takes part.
-template <int DP, int ROWS, int NS>
-__device__ __forceinline__ void attend(State<DP, ROWS>& st, const Query<DP, ROWS>& q, const uint8_t* sk,
-                                       const uint8_t* sv, const uint32_t* pk, const uint32_t* pv, int tile_rows,
-                                       uint32_t valid, float scale_log2) {
-  constexpr int NG = DP / 32;
+// NS subtiles of 16 keys each: keys and values at `sk`, `sv`, `tile_rows` rows per
+// swizzled tile; bit i of `valid` says whether key i takes part.
+template <int DP, int NS>
+__device__ __forceinline__ void attend_bf16(State<DP, kBf16Heads>& st, const Query<DP, kBf16Heads>& q,
+                                            const uint8_t* sk, const uint8_t* sv, int tile_rows, uint32_t valid,
+                                            float scale_log2) {
   const int lane = threadIdx.x & 31, n = lane >> 2, t = lane & 3;
-  const int group = n & (NG - 1);  // of this row, where rows are (head, group)
   constexpr uint32_t kAll = NS == 2 ? 0xffffffffu : 0xffffu;
   float s[2 * NS][2];  // scores of columns 2t, 2t + 1 of each 8 keys, row n
 #pragma unroll
   for (int i = 0; i < 2 * NS; ++i) {
     const int r = i * 8 + n;
-    if constexpr (ROWS == kBf16Heads) {
-      float acc[4] = {0.f, 0.f, 0.f, 0.f};
+    float acc[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int a = 0; a < DP / 64; ++a) {
+    for (int a = 0; a < DP / 64; ++a) {
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          const uint4 w = *swz(sk + a * tile_rows * 128, r, 2 * t + c);
-          mma16816(acc, q.a[a * 4 + c * 2][0], 0u, q.a[a * 4 + c * 2][1], 0u, w.x, w.y);
-          mma16816(acc, q.a[a * 4 + c * 2 + 1][0], 0u, q.a[a * 4 + c * 2 + 1][1], 0u, w.z, w.w);
-        }
-      }
-      s[i][0] = acc[0];
-      s[i][1] = acc[1];
-    } else {
-      uint32_t w[NG];
-      const uint8_t* p = sk + r * (DP / 2) + t * (DP / 8);
-      if constexpr (NG == 2) {
-        const uint2 u = *reinterpret_cast<const uint2*>(p);
-        w[0] = u.x, w[1] = u.y;
-      } else {
-        const uint4 u = *reinterpret_cast<const uint4*>(p);
-        w[0] = u.x, w[1] = u.y, w[2] = u.z, w[3] = u.w;
-      }
-      const uint32_t* par = pk + (i * 8 + 2 * t) * NG;  // of the keys of columns 2t, 2t + 1
-      if constexpr (ROWS == kPackedGroups) {
-        float acc[4] = {q.off[0] * -128.f, q.off[0] * -128.f, 0.f, 0.f};
-#pragma unroll
-        for (int g = 0; g < NG; ++g) {  // rows of other groups hold zeros there
-          mma16816(acc, q.a[2 * g][0], 0u, q.a[2 * g][1], 0u, code_pair(w[g], 0), code_pair(w[g], 1));
-          mma16816(acc, q.a[2 * g + 1][0], 0u, q.a[2 * g + 1][1], 0u, code_pair(w[g], 2), code_pair(w[g], 3));
-        }
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const uint32_t x = par[e * NG + group];
-          float v = fmaf(param_step(x), acc[e], param_low(x) * q.off[0]);
-          v += __shfl_xor_sync(0xffffffff, v, 4);  // the groups of a head lie in neighbouring rows
-          if (NG == 4) v += __shfl_xor_sync(0xffffffff, v, 8);
-          s[i][e] = v;
-        }
-      } else {
-        // least values times query sums: k-slots (2t, 2t + 1) and (2t + 8, 2t + 9)
-        float base[4] = {0.f, 0.f, 0.f, 0.f};
-        const uint2 lw = *reinterpret_cast<const uint2*>(pk + r * NG + (NG == 4 ? 2 * (t & 1) : 0));
-        const uint32_t lows = __byte_perm(lw.x, lw.y, 0x7632);
-        mma16816(base, q.sum[0], 0u, q.sum[1], 0u, lows, NG == 4 && t < 2 ? lows : 0u);
-        s[i][0] = base[0];
-        s[i][1] = base[1];
-        uint32_t step[2][NG];
-#pragma unroll
-        for (int e = 0; e < 2; ++e)
-#pragma unroll
-          for (int g = 0; g < NG; g += 2) {
-            const uint2 x = *reinterpret_cast<const uint2*>(par + e * NG + g);
-            step[e][g] = x.x, step[e][g + 1] = x.y;
-          }
-#pragma unroll
-        for (int g = 0; g < NG; ++g) {
-          float acc[4] = {q.off[g], q.off[g], 0.f, 0.f};
-          mma16816(acc, q.a[2 * g][0], 0u, q.a[2 * g][1], 0u, code_pair(w[g], 0), code_pair(w[g], 1));
-          mma16816(acc, q.a[2 * g + 1][0], 0u, q.a[2 * g + 1][1], 0u, code_pair(w[g], 2), code_pair(w[g], 3));
-          s[i][0] = fmaf(param_step(step[0][g]), acc[0], s[i][0]);
-          s[i][1] = fmaf(param_step(step[1][g]), acc[1], s[i][1]);
-        }
+      for (int c = 0; c < 2; ++c) {
+        const uint4 w = *swz(sk + a * tile_rows * 128, r, 2 * t + c);
+        mma16816(acc, q.a[a * 4 + c * 2][0], 0u, q.a[a * 4 + c * 2][1], 0u, w.x, w.y);
+        mma16816(acc, q.a[a * 4 + c * 2 + 1][0], 0u, q.a[a * 4 + c * 2 + 1][1], 0u, w.z, w.w);
       }
     }
+    s[i][0] = acc[0];
+    s[i][1] = acc[1];
   }
   float mx = -INFINITY;
   if (valid != kAll) {
@@ -449,131 +423,265 @@ __device__ __forceinline__ void attend(State<DP, ROWS>& st, const Query<DP, ROWS
   for (int i = 0; i < 2 * NS; ++i) mx = fmaxf(mx, fmaxf(s[i][0], s[i][1]));
   mx = fmaxf(mx, __shfl_xor_sync(0xffffffff, mx, 1));
   mx = fmaxf(mx, __shfl_xor_sync(0xffffffff, mx, 2)) * scale_log2;
-  // As in the prompt's kernel a row keeps its reference maximum until a tile
-  // exceeds it by 8 (in log2).
-  const bool need = mx > st.m + 8.f;
-  if (__any_sync(0xffffffff, need)) {
-    const float c = need ? exp2f(st.m - mx) : 1.f;
-    if (need) st.m = mx;
-    st.l *= c;
+  if (__any_sync(0xffffffff, mx > st.m[0] + 8.f)) {
+    const float c = move_max(st.m[0], st.l[0], mx);
 #pragma unroll
     for (int i = 0; i < DP / 8; ++i)
 #pragma unroll
       for (int j = 0; j < 4; ++j) st.o[i][j] *= c;
-    if constexpr (ROWS != kBf16Heads) {
-#pragma unroll
-      for (int j = 0; j < 4; ++j) st.c[j] *= c;
-      st.low *= c;
-    }
   }
-  const float m_use = st.m == -INFINITY ? 0.f : st.m;
+  const float m_use = st.m[0] == -INFINITY ? 0.f : st.m[0];
 #pragma unroll
   for (int i = 0; i < 2 * NS; ++i)
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
       s[i][e] = exp2f(fmaf(s[i][e], scale_log2, -m_use));
-      st.l += s[i][e];
+      st.l[0] += s[i][e];
     }
 #pragma unroll
   for (int u = 0; u < NS; ++u) {
     const int r0 = u * 16 + 2 * t;  // this thread's keys: r0, r0 + 1, r0 + 8, r0 + 9
     const uint32_t in = valid >> r0;
-    // what lies in a masked row must not meet its zero probability
-    const bool on[4] = {(in & 1u) != 0, (in & 2u) != 0, (in & 0x100u) != 0, (in & 0x200u) != 0};
-    const float p[4] = {s[2 * u][0], s[2 * u][1], s[2 * u + 1][0], s[2 * u + 1][1]};
-    if constexpr (ROWS == kBf16Heads) {
-      uint32_t a0, a1, a2, a3;
-      split2(p[0], p[1], a0, a1);
-      split2(p[2], p[3], a2, a3);
+    uint32_t a0, a1, a2, a3;
+    split2(s[2 * u][0], s[2 * u][1], a0, a1);
+    split2(s[2 * u + 1][0], s[2 * u + 1][1], a2, a3);
 #pragma unroll
-      for (int a = 0; a < DP / 64; ++a) {
-        const uint8_t* tile = sv + a * tile_rows * 128;
-        uint4 x[4] = {*swz(tile, r0, n), *swz(tile, r0 + 1, n), *swz(tile, r0 + 8, n), *swz(tile, r0 + 9, n)};
-        if (valid != kAll) {
-#pragma unroll
-          for (int j = 0; j < 4; ++j)
-            if (!on[j]) x[j] = make_uint4(0, 0, 0, 0);
-        }
-        const uint32_t* w[4] = {&x[0].x, &x[1].x, &x[2].x, &x[3].x};
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          mma16816(st.o[a * 8 + 2 * j], a0, a1, a2, a3, __byte_perm(w[0][j], w[1][j], 0x5410),
-                   __byte_perm(w[2][j], w[3][j], 0x5410));
-          mma16816(st.o[a * 8 + 2 * j + 1], a0, a1, a2, a3, __byte_perm(w[0][j], w[1][j], 0x7632),
-                   __byte_perm(w[2][j], w[3][j], 0x7632));
-        }
+    for (int a = 0; a < DP / 64; ++a) {
+      const uint8_t* tile = sv + a * tile_rows * 128;
+      uint4 x[4] = {*swz(tile, r0, n), *swz(tile, r0 + 1, n), *swz(tile, r0 + 8, n), *swz(tile, r0 + 9, n)};
+      if (valid != kAll) {  // what lies in a masked row must not meet its zero probability
+        const uint4 z = make_uint4(0, 0, 0, 0);
+        if (!(in & 1u)) x[0] = z;
+        if (!(in & 2u)) x[1] = z;
+        if (!(in & 0x100u)) x[2] = z;
+        if (!(in & 0x200u)) x[3] = z;
       }
-    } else {
-      uint32_t w[4][NG / 2];
+      const uint32_t* w[4] = {&x[0].x, &x[1].x, &x[2].x, &x[3].x};
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const uint8_t* x = sv + (r0 + (j & 1) + (j >> 1) * 8) * (DP / 2) + n * (DP / 16);
-        if constexpr (NG == 2) {
-          w[j][0] = *reinterpret_cast<const uint32_t*>(x);
-        } else {
-          const uint2 y = *reinterpret_cast<const uint2*>(x);
-          w[j][0] = y.x, w[j][1] = y.y;
-        }
-      }
-      constexpr uint32_t kMinus128 = 0xc300c300u;
-      if constexpr (ROWS == kPackedGroups) {
-        float x[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          uint32_t par = pv[(r0 + (j & 1) + (j >> 1) * 8) * NG + group];
-          if (valid != kAll && !on[j]) par = 0u;
-          x[j] = p[j] * param_step(par);
-          st.low = fmaf(p[j], param_low(par), st.low);
-        }
-        uint32_t a0, a1, a2, a3;
-        split2(x[0], x[1], a0, a1);
-        split2(x[2], x[3], a2, a3);
-        mma16816(st.c, a0, a1, a2, a3, kMinus128, kMinus128);
-#pragma unroll
-        for (int g = 0; g < NG; ++g) {
-          const uint32_t lo = __byte_perm(w[0][g >> 1], w[1][g >> 1], (g & 1) ? 0x7632 : 0x5410);
-          const uint32_t hi = __byte_perm(w[2][g >> 1], w[3][g >> 1], (g & 1) ? 0x7632 : 0x5410);
-#pragma unroll
-          for (int j = 0; j < 4; ++j)  // meaningful in the rows of group g
-            mma16816(st.o[g * 4 + j], a0, a1, a2, a3, code_pair(lo, j), code_pair(hi, j));
-        }
-      } else {
-        uint32_t par[4][NG];
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-#pragma unroll
-          for (int g = 0; g < NG; g += 2) {
-            const uint2 x = *reinterpret_cast<const uint2*>(pv + (r0 + (j & 1) + (j >> 1) * 8) * NG + g);
-            par[j][g] = x.x, par[j][g + 1] = x.y;
-          }
-        // least values: columns n of the constant terms are groups n % NG
-        uint32_t a0, a1, a2, a3, lw[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          lw[j] = pv[(r0 + (j & 1) + (j >> 1) * 8) * NG + group];
-          if (valid != kAll && !on[j]) {
-            lw[j] = 0u;
-#pragma unroll
-            for (int g = 0; g < NG; ++g) par[j][g] = 0u;
-          }
-        }
-        split2(p[0], p[1], a0, a1);
-        split2(p[2], p[3], a2, a3);
-        mma16816(st.c, a0, a1, a2, a3, __byte_perm(lw[0], lw[1], 0x7632), __byte_perm(lw[2], lw[3], 0x7632));
-#pragma unroll
-        for (int g = 0; g < NG; ++g) {
-          split2(p[0] * param_step(par[0][g]), p[1] * param_step(par[1][g]), a0, a1);
-          split2(p[2] * param_step(par[2][g]), p[3] * param_step(par[3][g]), a2, a3);
-          const uint32_t col = group == g ? kMinus128 : 0u;
-          mma16816(st.c, a0, a1, a2, a3, col, col);
-          const uint32_t lo = __byte_perm(w[0][g >> 1], w[1][g >> 1], (g & 1) ? 0x7632 : 0x5410);
-          const uint32_t hi = __byte_perm(w[2][g >> 1], w[3][g >> 1], (g & 1) ? 0x7632 : 0x5410);
-#pragma unroll
-          for (int j = 0; j < 4; ++j) mma16816(st.o[g * 4 + j], a0, a1, a2, a3, code_pair(lo, j), code_pair(hi, j));
-        }
+        mma16816(st.o[a * 8 + 2 * j], a0, a1, a2, a3, __byte_perm(w[0][j], w[1][j], 0x5410),
+                 __byte_perm(w[2][j], w[3][j], 0x5410));
+        mma16816(st.o[a * 8 + 2 * j + 1], a0, a1, a2, a3, __byte_perm(w[0][j], w[1][j], 0x7632),
+                 __byte_perm(w[2][j], w[3][j], 0x7632));
       }
     }
   }
+}
+
+__device__ __forceinline__ uint32_t code_pair(uint32_t w, int i) {  // 128 + code, twice
+  return ((w >> (4 * i)) & 0x000f000fu) | 0x43004300u;
+}
+
+// The same over packed rows with parameters `pk`, `pv`. Thread (n, t) computes the
+// scores of keys n and n + 8 of a subtile for query rows 2t, 2t + 1.
+template <int DP, int ROWS, int NS>
+__device__ __forceinline__ void attend_packed(State<DP, ROWS>& st, const Query<DP, ROWS>& q, const uint8_t* sk,
+                                              const uint8_t* sv, const uint32_t* pk, const uint32_t* pv, uint32_t valid,
+                                              float scale_log2) {
+  using St = State<DP, ROWS>;
+  constexpr int NG = DP / 32, NH = St::kHeads;
+  const int lane = threadIdx.x & 31, n = lane >> 2, t = lane & 3;
+  const int g0 = (2 * t) & (NG - 1);  // packed groups: column 2t + e is group g0 + e
+  constexpr uint32_t kAll = NS == 2 ? 0xffffffffu : 0xffffu;
+  float s[NS][2][NH];  // [subtile][key n, n + 8][head]
+#pragma unroll
+  for (int u = 0; u < NS; ++u) {
+    uint32_t w[2][NG];
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const uint8_t* p = sk + (u * 16 + k * 8 + n) * (DP / 2) + t * (DP / 8);
+      if constexpr (NG == 2) {
+        const uint2 x = *reinterpret_cast<const uint2*>(p);
+        w[k][0] = x.x, w[k][1] = x.y;
+      } else {
+        const uint4 x = *reinterpret_cast<const uint4*>(p);
+        w[k][0] = x.x, w[k][1] = x.y, w[k][2] = x.z, w[k][3] = x.w;
+      }
+    }
+    auto step_of = [&](int g, int half, uint32_t (&a)[4]) {  // A operand: 16 keys x 16 channels of group g
+      a[0] = code_pair(w[0][g], 2 * half);
+      a[1] = code_pair(w[1][g], 2 * half);
+      a[2] = code_pair(w[0][g], 2 * half + 1);
+      a[3] = code_pair(w[1][g], 2 * half + 1);
+    };
+    const uint32_t* par = pk + (u * 16 + n) * NG;  // of key n; key n + 8: 8 NG further
+    if constexpr (ROWS == kPackedGroups) {
+      float acc[4] = {q.off[0][0] * -128.f, q.off[0][1] * -128.f, q.off[0][0] * -128.f, q.off[0][1] * -128.f};
+#pragma unroll
+      for (int kk = 0; kk < DP / 16; ++kk) {  // columns of other groups hold zeros there
+        uint32_t a[4];
+        step_of(kk >> 1, kk & 1, a);
+        mma16816(acc, a, q.a[kk][0], q.a[kk][1], acc[0], acc[1], acc[2], acc[3]);
+      }
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        const uint2 x = *reinterpret_cast<const uint2*>(par + k * 8 * NG + g0);
+        float v = fmaf(param_step(x.x), acc[2 * k], param_low(x.x) * q.off[0][0]) +
+                  fmaf(param_step(x.y), acc[2 * k + 1], param_low(x.y) * q.off[0][1]);
+        if (NG == 4) v += __shfl_xor_sync(0xffffffff, v, 1);  // the head's other two groups
+        s[u][k][0] = v;
+      }
+    } else {
+      // least values times query sums: k-slots (2t, 2t + 1) and (2t + 8, 2t + 9)
+      uint32_t low[4];
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        const uint2 x = *reinterpret_cast<const uint2*>(par + k * 8 * NG + (NG == 4 ? 2 * (t & 1) : 0));
+        low[k] = __byte_perm(x.x, x.y, 0x7632);
+        low[2 + k] = NG == 4 && t < 2 ? low[k] : 0u;
+      }
+      float sc[4];
+      mma16816(sc, low, q.sum[0], q.sum[1], 0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int g = 0; g < NG; ++g) {
+        float acc[4];
+        uint32_t a[4];
+        step_of(g, 0, a);
+        mma16816(acc, a, q.a[2 * g][0], q.a[2 * g][1], q.off[g][0], q.off[g][1], q.off[g][0], q.off[g][1]);
+        step_of(g, 1, a);
+        mma16816(acc, a, q.a[2 * g + 1][0], q.a[2 * g + 1][1], acc[0], acc[1], acc[2], acc[3]);
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          const float step = param_step(par[k * 8 * NG + g]);
+          sc[2 * k] = fmaf(step, acc[2 * k], sc[2 * k]);
+          sc[2 * k + 1] = fmaf(step, acc[2 * k + 1], sc[2 * k + 1]);
+        }
+      }
+#pragma unroll
+      for (int k = 0; k < 2; ++k)
+#pragma unroll
+        for (int e = 0; e < NH; ++e) s[u][k][e] = sc[2 * k + e];
+    }
+  }
+  const bool masked = valid != kAll;
+  if (masked) {
+#pragma unroll
+    for (int u = 0; u < NS; ++u)
+#pragma unroll
+      for (int k = 0; k < 2; ++k)
+        if (!((valid >> (u * 16 + k * 8 + n)) & 1u)) {
+#pragma unroll
+          for (int e = 0; e < NH; ++e) s[u][k][e] = -INFINITY;
+        }
+  }
+  float mx[NH], m_use[NH];
+  bool need = false;
+#pragma unroll
+  for (int e = 0; e < NH; ++e) {
+    mx[e] = -INFINITY;
+#pragma unroll
+    for (int u = 0; u < NS; ++u) mx[e] = fmaxf(mx[e], fmaxf(s[u][0][e], s[u][1][e]));
+    mx[e] *= scale_log2;
+    need = need || mx[e] > st.m[e] + 8.f;
+  }
+  if (__any_sync(0xffffffff, need)) {  // only now the maxima of all keys are needed
+    float c[NH];
+#pragma unroll
+    for (int e = 0; e < NH; ++e) {
+#pragma unroll
+      for (int o = 4; o < 32; o <<= 1) mx[e] = fmaxf(mx[e], __shfl_xor_sync(0xffffffff, mx[e], o));
+      c[e] = move_max(st.m[e], st.l[e], mx[e]);
+    }
+    // the factor of output row n lies with the threads that hold column n
+    const float even = __shfl_sync(0xffffffff, c[0], n >> 1), odd = __shfl_sync(0xffffffff, c[NH - 1], n >> 1);
+    const float cn = (n & 1) ? odd : even;
+#pragma unroll
+    for (int i = 0; i < St::kTiles; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) st.o[i][j] *= cn;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) st.c[j] *= cn;
+#pragma unroll
+    for (int g = 0; g < (ROWS == kPackedHeads ? NG : 1); ++g)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) st.low[g][e] *= c[NH == 2 ? e : 0];
+  }
+#pragma unroll
+  for (int e = 0; e < NH; ++e) {
+    m_use[e] = st.m[e] == -INFINITY ? 0.f : st.m[e];
+#pragma unroll
+    for (int u = 0; u < NS; ++u)
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        s[u][k][e] = exp2f(fmaf(s[u][k][e], scale_log2, -m_use[e]));
+        st.l[e] += s[u][k][e];
+      }
+  }
+  constexpr uint32_t kMinus128 = 0xc300c300u;
+#pragma unroll
+  for (int u = 0; u < NS; ++u) {
+    const int r0 = u * 16 + 2 * t;  // values of this thread: keys r0, r0 + 1, r0 + 8, r0 + 9
+    uint32_t w[4][NG / 2];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const uint8_t* x = sv + (r0 + (j & 1) + (j >> 1) * 8) * (DP / 2) + n * (DP / 16);
+      if constexpr (NG == 2) {
+        w[j][0] = *reinterpret_cast<const uint32_t*>(x);
+      } else {
+        const uint2 y = *reinterpret_cast<const uint2*>(x);
+        w[j][0] = y.x, w[j][1] = y.y;
+      }
+    }
+    bool on[2] = {true, true};
+    if (masked) {  // what lies in a masked row must not meet its zero probability
+      on[0] = (valid >> (u * 16 + n)) & 1u;
+      on[1] = (valid >> (u * 16 + 8 + n)) & 1u;
+    }
+    const uint32_t* par = pv + (u * 16 + n) * NG;
+    auto values = [&](int g, int tile0, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3) {
+      const uint32_t lo = __byte_perm(w[0][g >> 1], w[1][g >> 1], (g & 1) ? 0x7632 : 0x5410);
+      const uint32_t hi = __byte_perm(w[2][g >> 1], w[3][g >> 1], (g & 1) ? 0x7632 : 0x5410);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) mma16816(st.o[tile0 + j], a0, a1, a2, a3, code_pair(lo, j), code_pair(hi, j));
+    };
+    if constexpr (ROWS == kPackedGroups) {
+      uint32_t hi[2], lo[2];
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        uint2 x = *reinterpret_cast<const uint2*>(par + k * 8 * NG + g0);
+        if (masked && !on[k]) x = make_uint2(0u, 0u);
+        const float p = s[u][k][0];
+        st.low[0][0] = fmaf(p, param_low(x.x), st.low[0][0]);
+        st.low[0][1] = fmaf(p, param_low(x.y), st.low[0][1]);
+        split2(p * param_step(x.x), p * param_step(x.y), hi[k], lo[k]);
+      }
+      const uint32_t a0 = transpose8(hi[0]), a1 = transpose8(lo[0]), a2 = transpose8(hi[1]), a3 = transpose8(lo[1]);
+      mma16816(st.c, a0, a1, a2, a3, kMinus128, kMinus128);
+#pragma unroll
+      for (int g = 0; g < NG; ++g) {  // into the rows of group g alone: one set of sums for all
+        const bool mine = (n & (NG - 1)) == g;
+        values(g, 0, mine ? a0 : 0u, mine ? a1 : 0u, mine ? a2 : 0u, mine ? a3 : 0u);
+      }
+    } else {
+#pragma unroll
+      for (int g = 0; g < NG; ++g) {
+        uint32_t hi[2], lo[2];
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          uint32_t x = par[k * 8 * NG + g];
+          if (masked && !on[k]) x = 0u;
+          const float step = param_step(x);
+#pragma unroll
+          for (int e = 0; e < 2; ++e) st.low[g][e] = fmaf(s[u][k][e], param_low(x), st.low[g][e]);
+          split2(s[u][k][0] * step, s[u][k][1] * step, hi[k], lo[k]);
+        }
+        const uint32_t a0 = transpose8(hi[0]), a1 = transpose8(lo[0]), a2 = transpose8(hi[1]), a3 = transpose8(lo[1]);
+        const uint32_t col = (n & (NG - 1)) == g ? kMinus128 : 0u;
+        mma16816(st.c, a0, a1, a2, a3, col, col);
+        values(g, g * 4, a0, a1, a2, a3);
+      }
+    }
+  }
+}
+
+template <int DP, int ROWS, int NS>
+__device__ __forceinline__ void attend(State<DP, ROWS>& st, const Query<DP, ROWS>& q, const uint8_t* sk,
+                                       const uint8_t* sv, const uint32_t* pk, const uint32_t* pv, int tile_rows,
+                                       uint32_t valid, float scale_log2) {
+  if constexpr (ROWS == kBf16Heads)
+    attend_bf16<DP, NS>(st, q, sk, sv, tile_rows, valid, scale_log2);
+  else
+    attend_packed<DP, ROWS, NS>(st, q, sk, sv, pk, pv, valid, scale_log2);
 }
 
 // Output channel of tile `tile`, column `n`.
@@ -683,9 +791,11 @@ __global__ void __launch_bounds__(kThreads, StepCfg<DP, ROWS>::kCtas)
         sum[g] += __shfl_xor_sync(0xffffffff, sum[g], 2);
       }
       if constexpr (ROWS == kPackedGroups) {
-        q.off[0] = 0.f;
+        float own = 0.f;  // zero but for the row's own group
 #pragma unroll
-        for (int g = 0; g < NG; ++g) q.off[0] += sum[g];  // zero but for the row's own group
+        for (int g = 0; g < NG; ++g) own += sum[g];
+#pragma unroll
+        for (int e = 0; e < 2; ++e) q.off[0][e] = __shfl_sync(0xffffffff, own, (2 * t + e) * 4);
       } else if constexpr (ROWS == kPackedHeads) {
         // three bf16 parts of each sum; thread t holds part t / 2 of groups 2 (t % 2), + 1
         // and, for t < 2, the third part (two groups: part t)
@@ -698,16 +808,20 @@ __global__ void __launch_bounds__(kThreads, StepCfg<DP, ROWS>::kCtas)
         q.sum[0] = part == 0 ? hi : part == 1 ? mid : (NG == 2 && part == 2) ? lo : 0u;
         q.sum[1] = NG == 4 && t < 2 ? lo : 0u;
 #pragma unroll
-        for (int g = 0; g < NG; ++g) q.off[g] = -128.f * sum[g];
+        for (int g = 0; g < NG; ++g)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) q.off[g][e] = -128.f * __shfl_sync(0xffffffff, sum[g], (2 * t + e) * 4);
       }
     }
   }
 
   State<DP, ROWS> st;
-  st.m = -INFINITY;
-  st.l = st.low = 0.f;
 #pragma unroll
-  for (int i = 0; i < DP / 8; ++i)
+  for (int e = 0; e < State<DP, ROWS>::kHeads; ++e) st.m[e] = -INFINITY, st.l[e] = 0.f;
+#pragma unroll
+  for (int g = 0; g < (ROWS == kPackedHeads ? NG : 1); ++g) st.low[g][0] = st.low[g][1] = 0.f;
+#pragma unroll
+  for (int i = 0; i < State<DP, ROWS>::kTiles; ++i)
 #pragma unroll
     for (int j = 0; j < 4; ++j) st.o[i][j] = 0.f;
 #pragma unroll
@@ -767,7 +881,7 @@ __global__ void __launch_bounds__(kThreads, StepCfg<DP, ROWS>::kCtas)
     const uint32_t* pk = reinterpret_cast<const uint32_t*>(src + 2 * C::kOperand);
     const uint32_t* pv = pk + KT * NG;
     const int row = first + (warp + i * kWarps) * KT;
-    constexpr int NS = KT % 32 == 0 ? 2 : 1;
+    constexpr int NS = C::kSub;
 #pragma unroll 1
     for (int u = 0; u < KT / (16 * NS); ++u) {
       const int r = row + u * 16 * NS;
@@ -787,36 +901,53 @@ __global__ void __launch_bounds__(kThreads, StepCfg<DP, ROWS>::kCtas)
   if (!ok && lane == 0)  // a wait expired: no copy may land after the CTA is gone
     for (int i = max(0, loaded - ST); i < loaded; ++i) mbar_wait(&full[i % ST], (i / ST) & 1, a.status, kTimeoutTmaFull);
 
-  // the keys of a row were spread over 4 lanes
-  st.l += __shfl_xor_sync(0xffffffff, st.l, 1);
-  st.l += __shfl_xor_sync(0xffffffff, st.l, 2);
-  float add[NG];  // what all channels of a group get
+  // Row n's m, l and constant terms, over all keys of the warp.
+  float row_m, row_l, add[NG];
 #pragma unroll
   for (int g = 0; g < NG; ++g) add[g] = 0.f;
-  if constexpr (ROWS == kPackedHeads) {
-    const float c0 = st.c[0] + st.c[2], c1 = st.c[1] + st.c[3];
+  if constexpr (ROWS == kBf16Heads) {  // keys were spread over 4 lanes
+    row_m = st.m[0];
+    row_l = st.l[0];
+    row_l += __shfl_xor_sync(0xffffffff, row_l, 1);
+    row_l += __shfl_xor_sync(0xffffffff, row_l, 2);
+  } else {  // keys were spread over 8 groups of 4 lanes, query rows 2t, 2t + 1 over the 4
+    auto over_keys = [](float x) {
 #pragma unroll
-    for (int g = 0; g < NG; ++g) add[g] = __shfl_sync(0xffffffff, (g & 1) ? c1 : c0, (lane & 28) + (g >> 1));
-  } else if constexpr (ROWS == kPackedGroups) {
-    st.low += __shfl_xor_sync(0xffffffff, st.low, 1);
-    st.low += __shfl_xor_sync(0xffffffff, st.low, 2);
+      for (int o = 4; o < 32; o <<= 1) x += __shfl_xor_sync(0xffffffff, x, o);
+      return x;
+    };
+    auto to_row = [&](float even, float odd) {
+      even = __shfl_sync(0xffffffff, even, n >> 1);
+      odd = __shfl_sync(0xffffffff, odd, n >> 1);
+      return (n & 1) ? odd : even;
+    };
+    constexpr int kLast = State<DP, ROWS>::kHeads - 1;
+    row_m = to_row(st.m[0], st.m[kLast]);
+    row_l = to_row(over_keys(st.l[0]), over_keys(st.l[kLast]));
+    if constexpr (ROWS == kPackedHeads) {
+      const float c0 = st.c[0] + st.c[2], c1 = st.c[1] + st.c[3];
 #pragma unroll
-    for (int g = 0; g < NG; ++g) add[g] = st.low + st.c[0] + st.c[2];
+      for (int g = 0; g < NG; ++g)
+        add[g] = to_row(over_keys(st.low[g][0]), over_keys(st.low[g][1])) +
+                 __shfl_sync(0xffffffff, (g & 1) ? c1 : c0, (lane & 28) + (g >> 1));
+    } else {
+      add[0] = to_row(over_keys(st.low[0][0]), over_keys(st.low[0][1])) + st.c[0] + st.c[2];
+    }
   }
   __syncthreads();  // every ring has been read
   float* join = reinterpret_cast<float*>(smem);  // [warp][row][DP + 2]: output, m, l
   if (row_head < heads) {
     float* row = join + (warp * kRows + row_head) * (DP + 2);
 #pragma unroll
-    for (int i = 0; i < DP / 8; ++i) {
-      if (ROWS == kPackedGroups && (i >> 2) != row_group) continue;  // another row's channels
-      const float c = C::kPacked ? add[i >> 2] : 0.f;
-      row[channel_of<DP, ROWS>(i, 2 * t)] = st.o[i][0] + st.o[i][2] + c;
-      row[channel_of<DP, ROWS>(i, 2 * t + 1)] = st.o[i][1] + st.o[i][3] + c;
+    for (int i = 0; i < State<DP, ROWS>::kTiles; ++i) {
+      const int tile = ROWS == kPackedGroups ? row_group * 4 + i : i;
+      const float c = C::kPacked ? add[ROWS == kPackedGroups ? 0 : i >> 2] : 0.f;
+      row[channel_of<DP, ROWS>(tile, 2 * t)] = st.o[i][0] + st.o[i][2] + c;
+      row[channel_of<DP, ROWS>(tile, 2 * t + 1)] = st.o[i][1] + st.o[i][3] + c;
     }
     if (t == 0 && (ROWS != kPackedGroups || row_group == 0)) {
-      row[DP] = st.m;
-      row[DP + 1] = st.l;
+      row[DP] = row_m;
+      row[DP + 1] = row_l;
     }
   }
   __syncthreads();
