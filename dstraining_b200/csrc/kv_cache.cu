@@ -468,9 +468,25 @@ __device__ __forceinline__ void attend_bf16(State<DP, kBf16Heads>& st, const Que
   }
 }
 
-__device__ __forceinline__ uint32_t code_pair(uint32_t w, int i) {  // 128 + code, twice
-  return ((w >> (4 * i)) & 0x000f000fu) | 0x43004300u;
-}
+// Codes i and i + 4 of a word as a bf16 pair of 128 + code: a shift, and one
+// three-input operation for mask and exponent (with both constants in registers;
+// as immediates they took one each).
+struct Codes {
+  uint32_t mask, exponent;
+  __device__ __forceinline__ Codes() {
+    asm volatile("mov.u32 %0, 0x000f000f;" : "=r"(mask));
+    asm volatile("mov.u32 %0, 0x43004300;" : "=r"(exponent));
+  }
+  __device__ __forceinline__ uint32_t first(uint32_t w) const {
+    uint32_t r;
+    asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(r) : "r"(w), "r"(mask), "r"(exponent));
+    return r;
+  }
+  __device__ __forceinline__ void all(uint32_t w, uint32_t (&pair)[4]) const {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) pair[i] = first(w >> (4 * i));
+  }
+};
 
 // The same over packed rows with parameters `pk`, `pv`. Thread (n, t) computes the
 // scores of keys n and n + 8 of a subtile for query rows 2t, 2t + 1.
@@ -481,6 +497,7 @@ __device__ __forceinline__ void attend_packed(State<DP, ROWS>& st, const Query<D
   using St = State<DP, ROWS>;
   constexpr int NG = DP / 32, NH = St::kHeads;
   const int lane = threadIdx.x & 31, n = lane >> 2, t = lane & 3;
+  const Codes codes;
   const int g0 = (2 * t) & (NG - 1);  // packed groups: column 2t + e is group g0 + e
   constexpr uint32_t kAll = NS == 2 ? 0xffffffffu : 0xffffu;
   float s[NS][2][NH];  // [subtile][key n, n + 8][head]
@@ -498,20 +515,23 @@ __device__ __forceinline__ void attend_packed(State<DP, ROWS>& st, const Query<D
         w[k][0] = x.x, w[k][1] = x.y, w[k][2] = x.z, w[k][3] = x.w;
       }
     }
-    auto step_of = [&](int g, int half, uint32_t (&a)[4]) {  // A operand: 16 keys x 16 channels of group g
-      a[0] = code_pair(w[0][g], 2 * half);
-      a[1] = code_pair(w[1][g], 2 * half);
-      a[2] = code_pair(w[0][g], 2 * half + 1);
-      a[3] = code_pair(w[1][g], 2 * half + 1);
+    // A operands of group g: 16 keys x its first and its last 16 channels
+    auto key_codes = [&](int g, uint32_t (&a)[4], uint32_t (&b)[4]) {
+      uint32_t x[4], y[4];
+      codes.all(w[0][g], x);
+      codes.all(w[1][g], y);
+      a[0] = x[0], a[1] = y[0], a[2] = x[1], a[3] = y[1];
+      b[0] = x[2], b[1] = y[2], b[2] = x[3], b[3] = y[3];
     };
     const uint32_t* par = pk + (u * 16 + n) * NG;  // of key n; key n + 8: 8 NG further
     if constexpr (ROWS == kPackedGroups) {
       float acc[4] = {q.off[0][0] * -128.f, q.off[0][1] * -128.f, q.off[0][0] * -128.f, q.off[0][1] * -128.f};
 #pragma unroll
-      for (int kk = 0; kk < DP / 16; ++kk) {  // columns of other groups hold zeros there
-        uint32_t a[4];
-        step_of(kk >> 1, kk & 1, a);
-        mma16816(acc, a, q.a[kk][0], q.a[kk][1], acc[0], acc[1], acc[2], acc[3]);
+      for (int g = 0; g < NG; ++g) {  // columns of other groups hold zeros there
+        uint32_t a[4], b[4];
+        key_codes(g, a, b);
+        mma16816(acc, a, q.a[2 * g][0], q.a[2 * g][1], acc[0], acc[1], acc[2], acc[3]);
+        mma16816(acc, b, q.a[2 * g + 1][0], q.a[2 * g + 1][1], acc[0], acc[1], acc[2], acc[3]);
       }
 #pragma unroll
       for (int k = 0; k < 2; ++k) {
@@ -535,11 +555,10 @@ __device__ __forceinline__ void attend_packed(State<DP, ROWS>& st, const Query<D
 #pragma unroll
       for (int g = 0; g < NG; ++g) {
         float acc[4];
-        uint32_t a[4];
-        step_of(g, 0, a);
+        uint32_t a[4], b[4];
+        key_codes(g, a, b);
         mma16816(acc, a, q.a[2 * g][0], q.a[2 * g][1], q.off[g][0], q.off[g][1], q.off[g][0], q.off[g][1]);
-        step_of(g, 1, a);
-        mma16816(acc, a, q.a[2 * g + 1][0], q.a[2 * g + 1][1], acc[0], acc[1], acc[2], acc[3]);
+        mma16816(acc, b, q.a[2 * g + 1][0], q.a[2 * g + 1][1], acc[0], acc[1], acc[2], acc[3]);
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
           const float step = param_step(par[k * 8 * NG + g]);
@@ -631,8 +650,11 @@ __device__ __forceinline__ void attend_packed(State<DP, ROWS>& st, const Query<D
     auto values = [&](int g, int tile0, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3) {
       const uint32_t lo = __byte_perm(w[0][g >> 1], w[1][g >> 1], (g & 1) ? 0x7632 : 0x5410);
       const uint32_t hi = __byte_perm(w[2][g >> 1], w[3][g >> 1], (g & 1) ? 0x7632 : 0x5410);
+      uint32_t x[4], y[4];
+      codes.all(lo, x);
+      codes.all(hi, y);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) mma16816(st.o[tile0 + j], a0, a1, a2, a3, code_pair(lo, j), code_pair(hi, j));
+      for (int j = 0; j < 4; ++j) mma16816(st.o[tile0 + j], a0, a1, a2, a3, x[j], y[j]);
     };
     if constexpr (ROWS == kPackedGroups) {
       uint32_t hi[2], lo[2];
