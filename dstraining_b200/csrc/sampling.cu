@@ -10,20 +10,23 @@
 // gives token -1 and logprob -inf.
 //
 // Drawing by the maximum of t + g needs no sorted order: whether a token is kept
-// is a question about the tokens before it, answered by one sum over the row. So
-// the winner among all candidates is taken first and then checked; a token that
-// is not kept rules out everything after it too, and the next winner is looked
-// for among what is left. With top_p = 0.9 nine of ten first winners stand. The
-// candidates are narrowed first by bounds that cost nothing: min_p; top_k by the
-// k-th largest of the threads' own maxima (a lower bound of the k-th largest
-// logit); top_p by the mass a token must have if V of its like are to count.
-// Only candidates' noise is read.
+// is a question about the tokens before it, answered by one sum. So the winner
+// among all candidates is taken first and then checked; a token that is not kept
+// rules out everything after it too, and the next winner is looked for among what
+// is left. With top_p = 0.9 nine of ten first winners stand. The candidates are
+// narrowed first by bounds that cost little: min_p; top_p by the mass a token must
+// have if V of its like are to count; top_k by a histogram of each thread's own
+// largest logits, whose k-th is a lower bound of the row's k-th. What top_k leaves
+// is a list; up to 256 entries are ranked against each other at once, which answers
+// everything in one round. Only candidates' noise is read.
 //
-// One CTA per row; the row is read once and stays in shared memory as fp32 t
-// (longer rows are read again from L2 in each pass). Bound by one SM's load rate
-// and by the passes over shared memory, not by HBM. Masses are summed as integers
-// of 2^-31 of the largest, so every sum and with it every choice is independent
-// of the order of the additions; logsumexp is an fp32 sum in a fixed order.
+// One CTA per row; the row is read once and stays in shared memory as fp32 (longer
+// rows are read again from L2 in each pass). t is divided out only for candidates;
+// the passes over the whole row work on x, of which t is a monotone function. Bound
+// by one SM's load rate, its passes over shared memory and the barriers between
+// them, not by HBM. Masses are summed as integers of 2^-31 of the largest, so every
+// sum and with it every choice is independent of the order of the additions;
+// logsumexp is an fp32 sum in a fixed order.
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/extension.h>
@@ -35,8 +38,9 @@ namespace sampling {
 
 constexpr int kThreads = 1024;
 constexpr int kWarps = kThreads / 32;
-constexpr int kMaxCached = 55296;  // t of a row in shared memory (216 KB)
-constexpr int kList = 1024;        // candidates kept as a list
+constexpr int kMaxCached = 52224;  // a row in shared memory (204 KB)
+constexpr int kList = 2048;        // candidates kept as a list
+constexpr int kRanked = 256;       // of a list ranked pair by pair
 constexpr int kBins = 256;
 
 struct Args {
@@ -77,8 +81,10 @@ struct Scratch {
   unsigned long long u[kWarps];
   uint32_t hist[kBins];
   uint32_t pick[4];
+  uint32_t weights[kRanked];
   int list_n;
   int list[kList];
+  float list_t[kList];
 };
 
 __device__ __forceinline__ Best block_best(Best v, Scratch& s) {
@@ -100,6 +106,30 @@ __device__ __forceinline__ Best block_best(Best v, Scratch& s) {
     w.index = __shfl_xor_sync(0xffffffff, v.index, o);
     v = better(v, w);
   }
+  return v;
+}
+
+__device__ __forceinline__ float block_max(float v, Scratch& s) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffff, v, o));
+  __syncthreads();
+  if ((threadIdx.x & 31) == 0) s.f[threadIdx.x >> 5] = v;
+  __syncthreads();
+  v = s.f[threadIdx.x & 31];
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffff, v, o));
+  return v;
+}
+
+__device__ __forceinline__ float block_min(float v, Scratch& s) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v = fminf(v, __shfl_xor_sync(0xffffffff, v, o));
+  __syncthreads();
+  if ((threadIdx.x & 31) == 0) s.f[threadIdx.x >> 5] = v;
+  __syncthreads();
+  v = s.f[threadIdx.x & 31];
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v = fminf(v, __shfl_xor_sync(0xffffffff, v, o));
   return v;
 }
 
@@ -147,29 +177,43 @@ __device__ __forceinline__ float to_float(__nv_bfloat16 x) {
   return __bfloat162float(x);
 }
 
-// The row: t by index.
+// The row: x by index (NaN as -inf, one zero: keys order -0 below +0), and t. In
+// shared memory x starts `pad` floats in, so that the global row's 16-byte vectors
+// land on 16-byte boundaries; what is left of the first and last four is -inf.
 template <typename T, bool CACHED>
 struct Row {
   const T* x;
   float* cache;
   float temperature;
-  int V;
-  __device__ __forceinline__ float scaled(T v) const {
-    const float f = to_float(v);
-    const float t = temperature == 1.f ? f : __fdiv_rn(f, temperature);
-    return t != t ? -INFINITY : (t == 0.f ? 0.f : t);  // one zero: keys order -0 below +0
+  int V, head, pad;
+  __device__ __forceinline__ Row(const T* x_, float* cache_, float temperature_, int V_)
+      : x(x_), cache(cache_), temperature(temperature_), V(V_) {
+    head = min(V, static_cast<int>((16 - (reinterpret_cast<uintptr_t>(x) & 15)) % 16 / sizeof(T)));
+    pad = (4 - head % 4) % 4;
   }
-  __device__ __forceinline__ float operator()(int i) const { return CACHED ? cache[i] : scaled(x[i]); }
+  static __device__ __forceinline__ float clean(T v) {
+    return __fadd_rn(fmaxf(to_float(v), -INFINITY), 0.f);
+  }
+  __device__ __forceinline__ float t_of(float f) const {
+    if (temperature == 1.f) return f;
+    const float t = __fdiv_rn(f, temperature);
+    return t == 0.f ? 0.f : t;
+  }
+  __device__ __forceinline__ float operator()(int i) const { return CACHED ? cache[i + pad] : clean(x[i]); }
 
-  // Calls f(i, t) for each element of this thread, in the order of a fixed
-  // assignment of elements to threads, reading global memory in 16-byte vectors.
+  // The first pass: the row into shared memory, f(i, x) for each element of this
+  // thread, reading global memory in 16-byte vectors, several in flight.
   template <typename F>
   __device__ __forceinline__ void load(F&& f) const {
-    constexpr int N = 16 / sizeof(T), U = 4;
-    const int head = min(V, static_cast<int>((16 - (reinterpret_cast<uintptr_t>(x) & 15)) % 16 / sizeof(T)));
+    constexpr int N = 16 / sizeof(T), U = 6;
     const int vectors = (V - head) / N;
     const uint4* p = reinterpret_cast<const uint4*>(x + head);
-    if (threadIdx.x < head) f(threadIdx.x, scaled(x[threadIdx.x]));
+    auto one = [&](int i) {
+      const float v = clean(x[i]);
+      if (CACHED) cache[i + pad] = v;
+      f(i, v);
+    };
+    if (threadIdx.x < head) one(threadIdx.x);
     for (int v0 = threadIdx.x; v0 < vectors; v0 += U * kThreads) {
       uint4 w[U];
 #pragma unroll
@@ -179,12 +223,39 @@ struct Row {
       for (int u = 0; u < U; ++u)
         if (v0 + u * kThreads < vectors) {
           const T* e = reinterpret_cast<const T*>(&w[u]);
+          const int i = head + (v0 + u * kThreads) * N;
 #pragma unroll
-          for (int j = 0; j < N; ++j) f(head + (v0 + u * kThreads) * N + j, scaled(e[j]));
+          for (int j = 0; j < N; j += 4) {
+            const float4 v = make_float4(clean(e[j]), clean(e[j + 1]), clean(e[j + 2]), clean(e[j + 3]));
+            if (CACHED) *reinterpret_cast<float4*>(cache + i + pad + j) = v;
+            f(i + j, v.x), f(i + j + 1, v.y), f(i + j + 2, v.z), f(i + j + 3, v.w);
+          }
         }
     }
     const int tail = head + vectors * N + threadIdx.x;
-    if (tail < V) f(tail, scaled(x[tail]));
+    if (tail < V) one(tail);
+    if (CACHED && threadIdx.x < 4) {
+      if (threadIdx.x < pad) cache[threadIdx.x] = -INFINITY;
+      if ((V + pad + threadIdx.x) / 4 == (V + pad) / 4) cache[V + pad + threadIdx.x] = -INFINITY;
+    }
+  }
+
+  // A later pass: f(i, x) for each element of this thread. Also called with x = -inf
+  // for up to 3 indices on either side of the row.
+  template <typename F>
+  __device__ __forceinline__ void sweep(F&& f) const {
+    if (CACHED) {
+      const int groups = (V + pad + 3) >> 2;
+#pragma unroll 2
+      for (int g = threadIdx.x; g < groups; g += kThreads) {
+        const float4 v = reinterpret_cast<const float4*>(cache)[g];
+        const int i = g * 4 - pad;
+        f(i, v.x), f(i + 1, v.y), f(i + 2, v.z), f(i + 3, v.w);
+      }
+    } else {
+#pragma unroll 4
+      for (int i = threadIdx.x; i < V; i += kThreads) f(i, clean(x[i]));
+    }
   }
 };
 
@@ -199,18 +270,40 @@ struct Candidates {
   }
 };
 
-// f(i, t) over the row or over the listed candidates.
+// f(i, t) over the listed candidates, or over the row's elements from x = `from` on.
 template <typename R, typename F>
-__device__ __forceinline__ void each(const R& row, const Scratch& s, bool listed, F&& f) {
+__device__ __forceinline__ void each(const R& row, const Scratch& s, bool listed, float from, F&& f) {
   if (listed) {
-    if (threadIdx.x < s.list_n) {
-      const int i = s.list[threadIdx.x];
-      f(i, row(i));
-    }
+    for (int i = threadIdx.x; i < s.list_n; i += kThreads) f(s.list[i], s.list_t[i]);
   } else {
-#pragma unroll 4
-    for (int i = threadIdx.x; i < row.V; i += kThreads) f(i, row(i));
+    row.sweep([&](int i, float x) {
+      if (x >= from && static_cast<unsigned>(i) < static_cast<unsigned>(row.V)) f(i, row.t_of(x));
+    });
   }
+}
+
+// The elements that `take(i, x)` accepts (none of -inf) as a list; false if they
+// are too many.
+template <typename R, typename F>
+__device__ __forceinline__ bool make_list(const R& row, Scratch& s, F&& take) {
+  __syncthreads();
+  if (threadIdx.x == 0) s.list_n = 0;
+  __syncthreads();
+  row.sweep([&](int i, float x) {
+    if (take(i, x)) {  // one addition for the lanes that take together
+      const unsigned lanes = __activemask();
+      const int lane = threadIdx.x & 31, leader = __ffs(lanes) - 1;
+      int at = 0;
+      if (lane == leader) at = atomicAdd(&s.list_n, __popc(lanes));
+      at = __shfl_sync(lanes, at, leader) + __popc(lanes & ((1u << lane) - 1));
+      if (at < kList) {
+        s.list[at] = i;
+        s.list_t[at] = row.t_of(x);
+      }
+    }
+  });
+  __syncthreads();
+  return s.list_n <= kList;
 }
 
 // The k-th largest (k >= 1) of the keys in [lo, hi] that `each` and `key` give,
@@ -277,96 +370,216 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(const Args a) {
   const uint32_t top_k = (k64 <= 0 || k64 >= V) ? 0u : static_cast<uint32_t>(k64);
   const float top_p = a.top_p_rows ? a.top_p_rows[b] : a.top_p;
   const float min_p = a.min_p_rows ? a.min_p_rows[b] : a.min_p;
-  const Row<T, CACHED> row{static_cast<const T*>(a.logits) + b * a.row_stride, cache, greedy ? 1.f : temperature, V};
+  const Row<T, CACHED> row(static_cast<const T*>(a.logits) + b * a.row_stride, cache, greedy ? 1.f : temperature, V);
   const float* gumbel = a.gumbel + b * a.gumbel_stride;
 
-  // the row, its first token, and each thread's largest t
-  Best first = {-INFINITY, V};
-  row.load([&](int i, float t) {
-    if (CACHED) cache[i] = t;
-    first = better(first, Best{t, i});
-  });
-  const float own_max = first.score;
-  first = block_best(first, s);  // also orders the cache's writes before the reads below
-  const float max = first.score;
-  if (max == -INFINITY) {
+  // the row, its largest logit, and each thread's own
+  float own_max = -INFINITY;
+  row.load([&](int, float x) { own_max = fmaxf(own_max, x); });
+  const float x_max = block_max(own_max, s);  // also orders the cache's writes before the reads below
+  if (x_max == -INFINITY) {
     if (tid == 0) {
       a.token[b] = -1;
       a.logprob[b] = -INFINITY;
     }
     return;
   }
+  const float max = row.t_of(x_max);
+  const float per_x = 1.4426950408889634f / row.temperature;
+  const bool by_mass = !greedy && top_p < 1.f;
   float sum = 0.f;
   unsigned long long total = 0;
-  const bool by_mass = !greedy && top_p < 1.f;
-#pragma unroll 4
-  for (int i = tid; i < V; i += kThreads) {
-    const float e = mass_of(row(i), max);
-    sum += e;
-    if (by_mass) total += weight(e);
-  }
+  if (by_mass && !top_k)
+    row.sweep([&](int, float x) {
+      const float e = x == x_max ? 1.f : exp2f((x - x_max) * per_x);
+      sum += e;
+      total += weight(e);
+    });
+  else
+    row.sweep([&](int, float x) { sum += x == x_max ? 1.f : exp2f((x - x_max) * per_x); });
   sum = block_sum(sum, s);
-  if (by_mass) total = block_sum(total, s);
 
-  Best winner = first;
+  Best winner = {-INFINITY, V};  // of the kept
   if (!greedy) {
-    Candidates c = {-INFINITY, V, -3.402823466e38f};  // a logit of -inf is never drawn
-    bool listed = false;
-    auto among = [&](auto&& f) { each(row, s, listed, f); };
+    // no token below this x is kept (with room for the rounding of t and exp)
+    float from = -3.402823466e38f;  // a logit of -inf never is
+    const float room = 1e-3f * row.temperature + 1e-5f * fabsf(x_max);
+    if (min_p > 0.f) from = fmaxf(from, x_max + logf(min_p) * row.temperature - room);
+    Candidates c = {-INFINITY, V, -3.402823466e38f};
+    bool listed = false, done = false;
     if (top_k) {
-      // at least k threads have a maximum >= the k-th largest maximum
-      uint32_t low_key = kLowestKey, taken;
-      if (top_k <= kThreads) {
-        const uint32_t mine = key_of(own_max);
-        low_key = select_key(s, kLowestKey, key_of(max), top_k, &taken, [&](auto&& f) { f(tid, own_max); },
-                             [&](int, float, uint32_t& u) { u = mine; return true; });
-      }
-      __syncthreads();
-      if (tid == 0) s.list_n = 0;
-      __syncthreads();
-      if (top_k <= kThreads) {
-#pragma unroll 4
-        for (int i = tid; i < V; i += kThreads)
-          if (key_of(row(i)) >= low_key) {
-            const int at = atomicAdd(&s.list_n, 1);
-            if (at < kList) s.list[at] = i;
+      // Bins of x, from the largest down, holding each thread's `m` largest: where
+      // k of those are reached, so are k of the row. One bin more than that, as
+      // different x may share a t.
+      const int m = top_k <= 256 ? 1 : 4;
+      float own[4] = {own_max, -INFINITY, -INFINITY, -INFINITY};
+      if (m > 1) {
+        own[0] = -INFINITY;
+        row.sweep([&](int, float x) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const float up = fmaxf(own[j], x);
+            x = fminf(own[j], x);
+            own[j] = up;
           }
-        __syncthreads();
-        listed = s.list_n <= kList;
-      }
-      const uint32_t key_k = select_key(s, low_key, key_of(max), top_k, &taken, among,
-                                        [&](int, float t, uint32_t& u) { u = key_of(t); return true; });
-      int last_index = V;
-      if (taken) {  // some of the equal values at the end, lowest index first
-        uint32_t rest;
-        const uint32_t u = select_key(s, 0u, static_cast<uint32_t>(V - 1), taken, &rest, among,
-                                      [&](int i, float t, uint32_t& v) {
-                                        v = static_cast<uint32_t>(V - 1 - i);
-                                        return key_of(t) == key_k;
-                                      });
-        last_index = V - 1 - static_cast<int>(u) + 1;
-      }
-      // the order's prefix ends at key_k, last_index
-      const uint32_t bits = (key_k & 0x80000000u) ? key_k & 0x7fffffffu : ~key_k;
-      c.bound = __uint_as_float(bits);
-      c.bound_index = last_index;
-      if (by_mass) {
-        total = 0;
-        among([&](int i, float t) {
-          if (c.has(t, i)) total += weight(mass_of(t, max));
         });
-        total = block_sum(total, s);
+      }
+      float least = own[0];
+#pragma unroll
+      for (int j = 1; j < 4; ++j)
+        if (j < m && own[j] > -INFINITY) least = own[j];
+      const float x_min = block_min(least > -INFINITY ? least : x_max, s);
+      const float bins = (kBins - 1) / (x_max - x_min);
+      if (x_max > x_min && bins < 3e38f && x_max < INFINITY && top_k <= 1024) {
+        auto bin = [&](float x) { return static_cast<int>(fminf((x_max - x) * bins, kBins - 1.f)); };
+        if (tid < kBins) s.hist[tid] = 0;
+        if (tid == 0) s.pick[0] = kBins;
+        __syncthreads();
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (j < m && own[j] > -INFINITY) atomicAdd(&s.hist[bin(own[j])], 1u);
+        __syncthreads();
+        if (tid < 32) {
+          uint32_t h[8], n = 0;
+#pragma unroll
+          for (int j = 0; j < 8; ++j) n += h[j] = s.hist[tid * 8 + j];
+          uint32_t upto = n;
+#pragma unroll
+          for (int o = 1; o < 32; o <<= 1) {
+            const uint32_t up = __shfl_up_sync(0xffffffff, upto, o);
+            if (tid >= o) upto += up;
+          }
+          uint32_t before = upto - n;
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            if (before < top_k && before + h[j] >= top_k) s.pick[0] = tid * 8 + j;
+            before += h[j];
+          }
+        }
+        __syncthreads();
+        const int last = static_cast<int>(s.pick[0]) + 1;
+        // the last bin holds everything below x_min too
+        // (top_p needs the mass of all k, so min_p does not thin them here)
+        if (last < kBins - 1) {
+          // everything with bin(x) <= last, and what rounding adds
+          const float end = x_max - static_cast<float>(last + 1) / bins * 1.00001f - 1e-6f * fabsf(x_max);
+          const float low = by_mass ? fmaxf(end, -3.402823466e38f) : fmaxf(end, from);
+          listed = make_list(row, s, [&](int, float x) { return x >= low; });
+        }
+      }
+      const int n = s.list_n;
+      if (listed && n <= kRanked) {
+        // few: each against all
+        if (tid < n) s.weights[tid] = static_cast<uint32_t>(weight(mass_of(s.list_t[tid], max)));
+        __syncthreads();
+        // four neighbouring threads a candidate, a quarter of the others each
+        const int mine = tid >> 2;
+        const bool on = mine < n;
+        const int i = on ? s.list[mine] : V;
+        const float t = on ? s.list_t[mine] : INFINITY;
+        uint32_t rank = 0;
+        unsigned long long before = 0;
+#pragma unroll 4
+        for (int j = tid & 3; j < n; j += 4) {
+          const float u = s.list_t[j];
+          const bool is = u > t || (u == t && s.list[j] < i);
+          const uint32_t w = s.weights[j];
+          rank += is;
+          before += is ? w : 0u;
+        }
+#pragma unroll
+        for (int o = 1; o < 4; o <<= 1) {
+          rank += __shfl_xor_sync(0xffffffff, rank, o);
+          before += __shfl_xor_sync(0xffffffff, before, o);
+        }
+        const bool owner = on && (tid & 3) == 0 && rank < top_k;
+        if (by_mass) total = block_sum(owner ? static_cast<unsigned long long>(s.weights[mine]) : 0ull, s);
+        if (owner && mass_of(t, max) >= min_p &&
+            (!by_mass || before == 0 || static_cast<float>(before) < top_p * static_cast<float>(total))) {
+          const float g = t + __ldg(gumbel + i);
+          winner = Best{g == g ? g : -INFINITY, i};
+        }
+        winner = block_best(winner, s);
+        done = true;
+      } else {
+        const float all = -INFINITY;
+        uint32_t taken;
+        auto among = [&](auto&& f) { each(row, s, listed, all, f); };
+        const uint32_t key_k = select_key(s, kLowestKey, key_of(max), min(top_k, static_cast<uint32_t>(listed ? n : V)),
+                                          &taken, among, [&](int, float t, uint32_t& u) { u = key_of(t); return true; });
+        int last_index = V;
+        if (taken) {  // some of the equal values at the end, lowest index first
+          uint32_t rest;
+          const uint32_t u = select_key(s, 0u, static_cast<uint32_t>(V - 1), taken, &rest, among,
+                                        [&](int i, float t, uint32_t& v) {
+                                          v = static_cast<uint32_t>(V - 1 - i);
+                                          return key_of(t) == key_k;
+                                        });
+          last_index = V - static_cast<int>(u);
+        }
+        // the order's prefix ends at key_k, last_index
+        const uint32_t bits = (key_k & 0x80000000u) ? key_k & 0x7fffffffu : ~key_k;
+        c.bound = __uint_as_float(bits);
+        c.bound_index = last_index;
+        if (by_mass) {
+          total = 0;
+          among([&](int i, float t) {
+            if (c.has(t, i)) total += weight(mass_of(t, max));
+          });
+        }
+      }
+    }
+    if (by_mass && !done) {
+      total = block_sum(total, s);
+      // V tokens of less than this cannot add up to the mass that top_p leaves out
+      const float tiny = (1.f - top_p) * (static_cast<float>(total) * 4.656612873e-10f) / static_cast<float>(V);
+      if (tiny > 0.f) from = fmaxf(from, x_max + logf(tiny) * row.temperature - room);
+      const float bins = (kBins - 1) / (x_max - from);
+      if (!top_k && bins > 0.f && bins < 3e38f) {
+        // Masses by bins of x from the largest down, rounded down: where they reach
+        // what is wanted the kept tokens end, or before. One bin more, as different x
+        // may share a t.
+        const float unit = 2147483648.f / static_cast<float>(V);  // no bin overflows
+        if (tid < kBins) s.hist[tid] = 0;
+        if (tid == 0) s.pick[0] = kBins;
+        __syncthreads();
+        row.sweep([&](int, float x) {
+          if (x >= from) {
+            const uint32_t w = __float2uint_rz((x == x_max ? 1.f : exp2f((x - x_max) * per_x)) * unit);
+            if (w) atomicAdd(&s.hist[static_cast<int>(fminf((x_max - x) * bins, kBins - 1.f))], w);
+          }
+        });
+        __syncthreads();
+        if (tid < 32) {
+          unsigned long long sum = 0;
+#pragma unroll
+          for (int j = 0; j < 8; ++j) sum += s.hist[tid * 8 + j];
+          unsigned long long upto = sum;
+#pragma unroll
+          for (int o = 1; o < 32; o <<= 1) {
+            const unsigned long long up = __shfl_up_sync(0xffffffff, upto, o);
+            if (tid >= o) upto += up;
+          }
+          unsigned long long before = upto - sum;
+          const float enough = top_p * static_cast<float>(total) * 1.00001f / static_cast<float>(V);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            const unsigned long long after = before + s.hist[tid * 8 + j];
+            if (static_cast<float>(before) < enough && static_cast<float>(after) >= enough) s.pick[0] = tid * 8 + j;
+            before = after;
+          }
+        }
+        __syncthreads();
+        const int last = static_cast<int>(s.pick[0]) + 1;
+        if (last < kBins)
+          from = fmaxf(from, x_max - static_cast<float>(last + 1) / bins * 1.00001f - 1e-6f * fabsf(x_max));
+        listed = make_list(row, s, [&](int, float x) { return x >= from; });
       }
     }
     const float wanted = by_mass ? top_p * static_cast<float>(total) : 0.f;
-    if (by_mass) {
-      // V tokens of less than this cannot add up to the mass that top_p leaves out
-      const float tiny = (1.f - top_p) * (static_cast<float>(total) * 4.656612873e-10f) / static_cast<float>(V);
-      if (tiny > 0.f) c.least = fmaxf(c.least, max + logf(tiny) - 1e-3f);
-    }
-    for (int tries = 0;; ++tries) {
+    while (!done) {
       Best w = {-INFINITY, V};
-      among([&](int i, float t) {
+      each(row, s, listed, from, [&](int i, float t) {
         if (c.has(t, i) && mass_of(t, max) >= min_p) {
           const float g = t + __ldg(gumbel + i);
           w = better(w, Best{g == g ? g : -INFINITY, i});
@@ -375,21 +588,36 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(const Args a) {
       w = block_best(w, s);
       if (w.index >= V) break;  // nothing but the first token
       winner = w;
-      if (!by_mass || w.index == first.index) break;
-      const float t_w = row(w.index);
-      unsigned long long before = 0;
-      among([&](int i, float t) {
-        if (t > t_w || (t == t_w && i < w.index)) before += weight(mass_of(t, max));
+      if (!by_mass) break;
+      const float t_w = row.t_of(row(w.index));
+      unsigned long long before = 0, count = 0;
+      each(row, s, listed, from, [&](int i, float t) {
+        if (t > t_w || (t == t_w && i < w.index)) {
+          before += weight(mass_of(t, max));
+          ++count;
+        }
       });
       before = block_sum(before, s);
-      if (static_cast<float>(before) < wanted) break;
-      winner = first;
+      if (before == 0 || static_cast<float>(before) < wanted) break;
+      winner = Best{-INFINITY, V};
       c.bound = t_w;  // out, and with it everything after it
       c.bound_index = w.index;
+      if (!listed) {
+        count = block_sum(count, s);
+        if (count <= kList)
+          listed = make_list(row, s, [&](int i, float x) { return x >= from && c.has(row.t_of(x), i); });
+      }
     }
   }
+  if (winner.index >= V) {  // greedy, or nothing else is kept: the first token of the order
+    row.sweep([&](int i, float x) {
+      // different x may share the largest t, near one another
+      if (x == x_max || (x >= x_max - 1e-5f * fabsf(x_max) && row.t_of(x) == max)) winner = better(winner, Best{0.f, i});
+    });
+    winner = block_best(winner, s);
+  }
   if (tid == 0) {
-    const float t = row(winner.index);
+    const float t = row.t_of(row(winner.index));
     a.token[b] = winner.index;
     a.logprob[b] = (t == max ? 0.f : t - max) - static_cast<float>(log(static_cast<double>(sum)));
   }
@@ -399,8 +627,9 @@ template <typename T>
 void launch(const Args& a, int B) {
   auto st = at::cuda::getCurrentCUDAStream();
   if (a.V <= kMaxCached) {
-    const int smem = a.V * 4;
-    C10_CUDA_CHECK(cudaFuncSetAttribute(sample_kernel<T, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxCached * 4));
+    const int smem = (a.V + 8) * 4;
+    C10_CUDA_CHECK(cudaFuncSetAttribute(sample_kernel<T, true>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                        (kMaxCached + 8) * 4));
     sample_kernel<T, true><<<B, kThreads, smem, st>>>(a);
   } else {
     sample_kernel<T, false><<<B, kThreads, 0, st>>>(a);
