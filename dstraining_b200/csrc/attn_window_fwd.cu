@@ -45,7 +45,8 @@ __global__ void __launch_bounds__(kThreads, 2)
   uint64_t* s_full = bars + 5;  // [2]
   uint64_t* p_full = bars + 7;  // [2]
   uint64_t* o_full = bars + 9;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 10);
+  uint64_t* o_last = bars + 10;  // the product of the last block
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 11);
 
   const int q0 = (gridDim.x - 1 - blockIdx.x) * 128;
   const int h = blockIdx.y, b = blockIdx.z, hk = h / s.G;
@@ -72,6 +73,7 @@ __global__ void __launch_bounds__(kThreads, 2)
       mbar_init(&p_full[i], 256);
     }
     mbar_init(o_full, 1);
+    mbar_init(o_last, 1);
     fence_barrier_init();
   }
   if (warp == 0) {  // the first copies travel while TMEM is allocated
@@ -117,7 +119,7 @@ __global__ void __launch_bounds__(kThreads, 2)
       for (int kk = 0; kk < 4; ++kk)  // O (+)= P V_j; k-step kk: columns of the half that computed it
         mma_ts(el, tmem + C::kO, tmem + 64 * (j & 1) + (kk >> 1) * 32 + (kk & 1) * 8, v + ((kk * 2048) >> 4), id_o,
                (j > 0 || kk > 0) ? 1u : 0u);
-      mma_commit(el, o_full);
+      mma_commit(el, j + 1 < n ? o_full : o_last);
       if (j + 2 < n) {  // V_j, and the buffer of S_j and P_j, are free once this is done
         ok = warp_wait(o_full, j & 1, s.status, kTimeoutTmemFull);
         if (ok) load_v(el);
@@ -190,7 +192,7 @@ __global__ void __launch_bounds__(kThreads, 2)
     red[256 + half * 128 + r] = l;
     pair_any(1 + quad, false);
     l += red[256 + (half ^ 1) * 128 + r];
-    if (__all_sync(0xffffffff, ok && mbar_wait(o_full, (n - 1) & 1, s.status, kTimeoutTmemFull))) {
+    if (__all_sync(0xffffffff, ok && mbar_wait(o_last, 0, s.status, kTimeoutTmemFull))) {
       tc_fence_after();
       const float inv = 1.f / l;
 #pragma unroll

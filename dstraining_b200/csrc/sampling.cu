@@ -579,12 +579,29 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(const Args a) {
     const float wanted = by_mass ? top_p * static_cast<float>(total) : 0.f;
     while (!done) {
       Best w = {-INFINITY, V};
-      each(row, s, listed, from, [&](int i, float t) {
-        if (c.has(t, i) && mass_of(t, max) >= min_p) {
-          const float g = t + __ldg(gumbel + i);
-          w = better(w, Best{g == g ? g : -INFINITY, i});
+      auto consider = [&](int i, float t, float g) {
+        if (c.has(t, i) && (!(min_p > 0.f) || mass_of(t, max) >= min_p)) {
+          const float score = t + g;
+          w = better(w, Best{score == score ? score : -INFINITY, i});
         }
-      });
+      };
+      if (listed) {
+        for (int j = tid; j < s.list_n; j += kThreads) consider(s.list[j], s.list_t[j], __ldg(gumbel + s.list[j]));
+      } else {
+        constexpr int U = 8;  // noise of so many candidates in flight
+        for (int i0 = tid; i0 < V; i0 += U * kThreads) {
+          float x[U], g[U];
+#pragma unroll
+          for (int u = 0; u < U; ++u) {
+            const int i = i0 + u * kThreads;
+            x[u] = i < V ? row(i) : -INFINITY;
+            g[u] = x[u] >= from ? __ldg(gumbel + i) : 0.f;
+          }
+#pragma unroll
+          for (int u = 0; u < U; ++u)
+            if (x[u] >= from) consider(i0 + u * kThreads, row.t_of(x[u]), g[u]);
+        }
+      }
       w = block_best(w, s);
       if (w.index >= V) break;  // nothing but the first token
       winner = w;

@@ -211,6 +211,29 @@ def test_repeatable_and_on_another_stream():
     assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
 
 
+@pytest.mark.parametrize("D", [64, 128])
+def test_long_sequences_repeat_exactly(D):
+    """Enough tiles and blocks that waves of CTAs overlap in many ways: the same bits every time, and right."""
+    from dstraining_b200.ops.window import window_attention_qkv
+
+    W, S = 700, 5
+    q, k, v = _rand(1, 4001, 16, D, seed=1), _rand(1, 4001, 4, D, seed=2), _rand(1, 4001, 4, D, seed=3)
+    dout = _rand(1, 4001, 16, D, seed=4)
+    x = [t.requires_grad_() for t in (q, k, v)]
+
+    def once():
+        out = window_attention_qkv(*x, W, S)
+        return (out.detach(), *torch.autograd.grad(out, x, dout))
+
+    runs = [once() for _ in range(8)]
+    for other in runs[1:]:
+        assert all(torch.equal(a, b) for a, b in zip(runs[0], other))
+    for h in (0, 7):  # two query heads, and the key head of each
+        one = [t.detach()[:, :, i:i + 1] for t, i in ((q, h), (k, h // 4), (v, h // 4))]
+        want = _exact(*one, W, S)[0]
+        assert _err(runs[0][0][:, :, h:h + 1], want) < 2 * U
+
+
 def test_graph_capture():
     from dstraining_b200.ops.window import window_attention
 
