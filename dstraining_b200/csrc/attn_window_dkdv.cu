@@ -10,6 +10,12 @@
 // pairs of score buffers; at 64 two CTAs share the SM, one pair each. The scores
 // of a block overwrite P and dS of an earlier one, each as soon as its own product
 // is done, so the tensor core always has the other one to work on.
+//
+// 8192 tokens, 16 heads of 128, window 1024, 4 sinks: 191 us, 680 TFLOP/s of its 4
+// products (floor 80 us); 8 x 1024 tokens, 12 heads of 64, window 256: 57 us. An MMA
+// with N = 64 and A in shared memory is bound by reading A (3x its multiplications),
+// which makes about 1100 of the 2300 cycles a step at head size 128. One pair of
+// buffers and four warps took 637 us there.
 #include "attn_window.cuh"
 
 namespace dst {

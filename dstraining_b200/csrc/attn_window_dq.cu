@@ -6,6 +6,10 @@
 // Warp 0 copies and issues MMAs; the others (two threads a row, 32 key columns
 // each) compute dS. dP of the next block runs beside dQ += dS K, the next S after
 // it, so the tensor core has no gap of its own between blocks.
+//
+// 8192 tokens, 16 heads of 128, window 1024: 137 us, 710 TFLOP/s of its 3 products
+// (floor 60 us); 8 x 1024 tokens, 12 heads of 64, window 256: 39 us. Bound like
+// dK and dV by the two products with A in shared memory.
 #include "attn_window.cuh"
 
 namespace dst {

@@ -7,6 +7,14 @@
 // one. The two halves of a row only meet where its maximum may have to move: a row
 // keeps its reference maximum until a block exceeds it by 8 (in log2), so P stays
 // below 2^8 and in most blocks one barrier between two warps is all they exchange.
+//
+// 8192 tokens, 16 heads of 128, window 1024: 94 us, 690 TFLOP/s of the visible
+// pairs (floor 40 us of tensor time); 8 x 1024 tokens, 12 heads of 64, window 256:
+// 34 us. A block takes about 800 cycles of an SM: 512 of them the exponentials (16 a
+// cycle; at head size 128 the tensor core needs as much), the rest the chain from
+// scores to sums where two tiles do not fill each other's gaps; 3 to 5 thousand
+// cycles a tile go to start and end. Tried: blocks of 128 keys (121 us: one score
+// buffer, the chain is exposed), a thread per row (144 us).
 #include "attn_window.cuh"
 
 namespace dst {

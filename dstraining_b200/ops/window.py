@@ -6,7 +6,7 @@ Key ``j`` is visible to query ``i`` iff ``j <= i`` and (``i - j < window`` or
 ``T * (window + sinks)`` instead of ``T^2``, and decoding needs a cache of only
 ``sinks + window`` slots (:mod:`dstraining_b200.ops.kv_cache`).
 
-* CUDA bf16: the tcgen05 kernels of ``csrc/attn_window.cu``. Head sizes are
+* CUDA bf16: the tcgen05 kernels of ``csrc/attn_window_*.cu``. Head sizes are
   multiples of 8 up to 128; any sequence length runs as it is (no padding);
   query heads may share key heads; operands are read where they lie if their
   strides are multiples of 16 bytes (copied otherwise). Backward recomputes the

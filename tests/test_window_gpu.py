@@ -258,6 +258,40 @@ def test_nothing_to_do(shape):
     assert x[0].grad.shape == shape
 
 
+def test_model_trains_and_decodes():
+    """A GPT with a window: loss as in fp32 on the CPU (both layers round activations, loss ~ 5.6: a few u
+    relative), decoding over the rolling cache as the full forward pass (activations rounded at other
+    places: 16 u of the logits' norm; 4-bit rows: a step is 1/15 of a group's range)."""
+    from dstraining_b200.models.gpt import GPT, GPTConfig
+    from dstraining_b200.parallel.topology import SINGLE
+    from dstraining_b200.utils.generate import KVCache, generate
+
+    cfg = GPTConfig(vocab_size=257, block_size=256, n_layer=2, n_head=2, n_embd=128, attention_window=40,
+                    attention_sinks=2)
+    idx = torch.randint(0, 257, (2, 200), generator=torch.Generator().manual_seed(1))
+    model, oracle = GPT(cfg, SINGLE, seed=3).cuda().to(torch.bfloat16), GPT(cfg, SINGLE, seed=3)
+    _, loss = model(idx.cuda(), idx.cuda())
+    _, want = oracle(idx, idx)
+    loss.backward()
+    want.backward()
+    assert abs(loss.item() - want.item()) < 8 * U * want.item()
+    for (name, a), b in zip(model.named_parameters(), oracle.parameters()):
+        if b.grad.norm() > 1e-3:
+            assert _err(a.grad.cpu(), b.grad.double()) < 32 * U, name
+    model.eval()
+    seq = idx.cuda()
+    with torch.no_grad():
+        full = model(seq)[0][:, 100:, :257].double()
+        for bits, tol in ((16, 16 * U), (4, 0.2)):
+            cache = KVCache(model, 2, bits)
+            got = [cache.forward(seq[:, :101])] + [cache.forward(seq[:, t:t + 1]) for t in range(101, 200)]
+            assert _err(torch.stack(got, dim=1), full) < tol
+    g = lambda: torch.Generator(device="cuda").manual_seed(4)  # noqa: E731
+    a, b = (generate(model, seq[:, :50], 30, 0.8, 20, g(), top_p=0.9, min_p=0.01, cache_bits=4, device_sampling=True)
+            for _ in range(2))
+    assert a.shape == (2, 80) and torch.equal(a, b)
+
+
 def test_refusals():
     from dstraining_b200.ops import native
     from dstraining_b200.ops.window import window_attention, window_attention_qkv
