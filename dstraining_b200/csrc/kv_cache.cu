@@ -31,13 +31,14 @@
 // (above the rate of a copy: it only reads); 4 bits the same 109 us, 4.3 TB/s, bound by
 // the integer pipe that makes operands of the codes (417 instructions per 16 keys and
 // warp before mask and exponent went in together, 134 us); 16 sequences x 2 key heads
-// x 8 query heads x 16384 slots 54 us, 1.0 TB/s, the same with 8 rows' probabilities
-// per group on top; one sequence x 12 heads of 64 x 32768 slots 21 us, 1.5 TB/s; one
+// x 8 query heads x 16384 slots 49 us, 1.1 TB/s, the same with 8 rows' probabilities
+// per group on top; one sequence x 12 heads of 64 x 32768 slots 20 us, 1.5 TB/s; one
 // sequence x 12 heads x 700 slots in bf16 7 us, latency.
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/extension.h>
 
+#include <algorithm>
 #include <map>
 #include <string>
 
@@ -327,6 +328,7 @@ struct StepCfg {
   // the new token's row, laid out like a stage of 16 keys
   static constexpr int kNew = 2 * 16 * (kRowBytes + kParamBytes);
   static constexpr int kJoin = kWarps * kRows * (DP + 2) * 4;  // over the ring at the end
+  static constexpr int kMaxSplits = kRingBytes / (4 * kRows) - 1;  // their weights too
   static constexpr int kSmem = (kRingBytes > kJoin ? kRingBytes : kJoin) + kNew + kWarps * kStages * 8 + 16 + 1024;
   static constexpr int kCtas = !kPacked ? 2 : ROWS == kPackedGroups ? 4 : DP == 64 ? 4 : 3;  // per SM
   static constexpr int kSub = ROWS == kPackedHeads ? 1 : KT % 32 == 0 ? 2 : 1;  // subtiles of 16 keys at a time
@@ -1020,20 +1022,51 @@ __global__ void __launch_bounds__(kThreads, StepCfg<DP, ROWS>::kCtas)
   if (!*last_flag) return;
   __threadfence();
   const float* all = a.partial + unit * a.splits * (kRows * (DP + 2));
+  constexpr int kStep = kRows * (DP + 2);
+  if (active <= 8) {  // few splits: at once (6 splits of one sequence: 7.0 us against 7.9)
+    for (int i = threadIdx.x; i < heads * DP; i += kThreads) {
+      const int r = i / DP, d = i % DP;
+      const float* row = all + r * (DP + 2);
+      float m = -INFINITY, o = 0.f, l = 0.f;
+      for (int s = 0; s < active; ++s) m = fmaxf(m, __ldcg(row + s * kStep + DP));
+#pragma unroll 4
+      for (int s = 0; s < active; ++s) {
+        const float c = exp2f(__ldcg(row + s * kStep + DP) - m);
+        o += c * __ldcg(row + s * kStep + d);
+        l += c * __ldcg(row + s * kStep + DP + 1);
+      }
+      if (d < a.D) a.out[(static_cast<int64_t>(b) * a.Hk * a.G + h0 + r) * a.D + d] = __float2bfloat16(o / l);
+    }
+    return;
+  }
+  // many: the splits' weights first (a warp per query row), then the outputs, with
+  // the loads of several splits in flight (13 splits: 48.9 us against 53.9)
+  float* weight = join;                     // [row][split]
+  float* inverse = join + kRows * active;   // [row]
+  for (int r = warp; r < heads; r += kWarps) {
+    const float* row = all + r * (DP + 2) + DP;
+    float m = -INFINITY, l = 0.f;
+    for (int s = lane; s < active; s += 32) m = fmaxf(m, __ldcg(row + static_cast<int64_t>(s) * kStep));
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffff, m, o));
+    for (int s = lane; s < active; s += 32) {
+      const float c = exp2f(__ldcg(row + static_cast<int64_t>(s) * kStep) - m);
+      weight[r * active + s] = c;
+      l += c * __ldcg(row + static_cast<int64_t>(s) * kStep + 1);
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffff, l, o);
+    if (lane == 0) inverse[r] = 1.f / l;
+  }
+  __syncthreads();
   for (int i = threadIdx.x; i < heads * DP; i += kThreads) {
     const int r = i / DP, d = i % DP;
-    const float* row = all + r * (DP + 2);
-    constexpr int64_t kStep = kRows * (DP + 2);
-    float m = -INFINITY;
-    for (int s = 0; s < active; ++s) m = fmaxf(m, __ldcg(row + s * kStep + DP));
-    float o = 0.f, l = 0.f;
-#pragma unroll 4
-    for (int s = 0; s < active; ++s) {
-      const float c = exp2f(__ldcg(row + s * kStep + DP) - m);
-      o += c * __ldcg(row + s * kStep + d);
-      l += c * __ldcg(row + s * kStep + DP + 1);
-    }
-    if (d < a.D) a.out[(static_cast<int64_t>(b) * a.Hk * a.G + h0 + r) * a.D + d] = __float2bfloat16(o / l);
+    const float* row = all + r * (DP + 2) + d;
+    float o = 0.f;
+#pragma unroll 8
+    for (int s = 0; s < active; ++s) o += weight[r * active + s] * __ldcg(row + static_cast<int64_t>(s) * kStep);
+    if (d < a.D)
+      a.out[(static_cast<int64_t>(b) * a.Hk * a.G + h0 + r) * a.D + d] = __float2bfloat16(o * inverse[r]);
   }
 }
 
@@ -1225,7 +1258,7 @@ class KVCache {
   }
 
   // How many CTAs share the slots of one (sequence, key head): as many as fit on the
-  // GPU at once (a few more would run after all others: 57 us instead of 54 for 16
+  // GPU at once (a few more would run after all others: 57 us against 54 for 16
   // sequences of 2 key heads), each with at least one tile per warp.
   const Work& work_for(int64_t chunks, Rows rows) {
     auto it = work_.find(chunks);
@@ -1235,7 +1268,7 @@ class KVCache {
     dispatch_step(rows, [&](auto dp, auto rows_c) {
       using C = StepCfg<dp(), static_cast<int>(rows_c())>;
       const int64_t most = (slots_ + kWarps * C::KT - 1) / (kWarps * C::KT);
-      splits = std::min(most, std::max<int64_t>(1, C::kCtas * num_sms() / units));
+      splits = std::min({most, std::max<int64_t>(1, C::kCtas * num_sms() / units), int64_t(C::kMaxSplits)});
     });
     Work w = {static_cast<int>(splits), at::empty({units * splits * kRows * (DP_ + 2)}, pos_.options().dtype(at::kFloat)),
               at::zeros({units}, pos_.options().dtype(at::kInt))};

@@ -85,6 +85,9 @@ CASES = [
     (1, 18, 1, 128, 129, 1, 200, 16),
     (1, 2, 2, 64, 700, 4, 690, 16),  # split over CTAs, and joined
     (1, 2, 2, 128, 700, 4, 690, 4),
+    (1, 4, 2, 64, 5000, 4, 4990, 4),  # over more splits than are joined at once
+    (1, 8, 1, 128, 5000, 4, 4990, 4),
+    (1, 8, 1, 64, 5000, 1, 4000, 16),
 ]
 
 
