@@ -368,8 +368,8 @@ struct State {
   static constexpr int kTiles = ROWS == kPackedGroups ? 4 : DP / 8;
   float m[kHeads], l[kHeads];
   float o[kTiles][4];  // [tile]: 0, 1 high parts, 2, 3 low parts of the probabilities
-  float c[4];          // -128 sum p step: packed heads: of groups 2t, 2t + 1; packed groups: of the row's
-  float low[ROWS == kPackedHeads ? NG : 1][2];  // sum p low of (group,) query row 2t, 2t + 1
+  float c[4];          // packed groups: -128 sum p step of the row's group
+  float low[ROWS == kPackedHeads ? NG : 1][2];  // sum p low (packed heads: p (low - 128 step)) of query row 2t, 2t + 1
 };
 
 // The query rows as mma operands. Packed: also -128 times their sums over groups
@@ -637,7 +637,6 @@ __device__ __forceinline__ void attend_packed(State<DP, ROWS>& st, const Query<D
         st.l[e] += s[u][k][e];
       }
   }
-  constexpr uint32_t kMinus128 = 0xc300c300u;
 #pragma unroll
   for (int u = 0; u < NS; ++u) {
     const int r0 = u * 16 + 2 * t;  // values of this thread: keys r0, r0 + 1, r0 + 8, r0 + 9
@@ -679,6 +678,7 @@ __device__ __forceinline__ void attend_packed(State<DP, ROWS>& st, const Query<D
         split2(p * param_step(x.x), p * param_step(x.y), hi[k], lo[k]);
       }
       const uint32_t a0 = transpose8(hi[0]), a1 = transpose8(lo[0]), a2 = transpose8(hi[1]), a3 = transpose8(lo[1]);
+      constexpr uint32_t kMinus128 = 0xc300c300u;
       mma16816(st.c, a0, a1, a2, a3, kMinus128, kMinus128);
 #pragma unroll
       for (int g = 0; g < NG; ++g) {  // into the rows of group g alone: one set of sums for all
@@ -693,14 +693,14 @@ __device__ __forceinline__ void attend_packed(State<DP, ROWS>& st, const Query<D
         for (int k = 0; k < 2; ++k) {
           uint32_t x = par[k * 8 * NG + g];
           if (masked && !on[k]) x = 0u;
-          const float step = param_step(x);
+          // the group's own sum takes the bias back: one that the groups share would spread
+          // a group that stands for NaN over all of them
+          const float step = param_step(x), base = fmaf(-128.f, step, param_low(x));
 #pragma unroll
-          for (int e = 0; e < 2; ++e) st.low[g][e] = fmaf(s[u][k][e], param_low(x), st.low[g][e]);
+          for (int e = 0; e < 2; ++e) st.low[g][e] = fmaf(s[u][k][e], base, st.low[g][e]);
           split2(s[u][k][0] * step, s[u][k][1] * step, hi[k], lo[k]);
         }
         const uint32_t a0 = transpose8(hi[0]), a1 = transpose8(lo[0]), a2 = transpose8(hi[1]), a3 = transpose8(lo[1]);
-        const uint32_t col = (n & (NG - 1)) == g ? kMinus128 : 0u;
-        mma16816(st.c, a0, a1, a2, a3, col, col);
         values(g, g * 4, a0, a1, a2, a3);
       }
     }
@@ -958,11 +958,8 @@ __global__ void __launch_bounds__(kThreads, StepCfg<DP, ROWS>::kCtas)
     row_m = to_row(st.m[0], st.m[kLast]);
     row_l = to_row(over_keys(st.l[0]), over_keys(st.l[kLast]));
     if constexpr (ROWS == kPackedHeads) {
-      const float c0 = st.c[0] + st.c[2], c1 = st.c[1] + st.c[3];
 #pragma unroll
-      for (int g = 0; g < NG; ++g)
-        add[g] = to_row(over_keys(st.low[g][0]), over_keys(st.low[g][1])) +
-                 __shfl_sync(0xffffffff, (g & 1) ? c1 : c0, (lane & 28) + (g >> 1));
+      for (int g = 0; g < NG; ++g) add[g] = to_row(over_keys(st.low[g][0]), over_keys(st.low[g][1]));
     } else {
       add[0] = to_row(over_keys(st.low[0][0]), over_keys(st.low[0][1])) + st.c[0] + st.c[2];
     }

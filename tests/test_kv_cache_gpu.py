@@ -290,3 +290,20 @@ def test_refusals():
         cache.step(q, k, k, torch.tensor([1, 2], device="cuda", dtype=torch.int32))
     with pytest.raises(ValueError, match="pos must"):
         cache.step(q, k, k, torch.tensor([1, 2]))
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("G", [1, 3, 8, 20])
+@pytest.mark.parametrize("new", [False, True])
+def test_a_nan_stays_in_its_group_however_many_heads_share_it(G, D, new):
+    """One NaN channel: its 32 channels stand for NaN, in a held row as in the new one; the others stay finite."""
+    from dstraining_b200.ops.kv_cache import WindowCache
+
+    cache = WindowCache(1, 1, D, 40, 0, bits=4, device="cuda")
+    k, v = _rand(1, 30, 1, D, seed=1), _rand(1, 30, 1, D, seed=2)
+    q, k1, v1 = _rand(1, G, D, seed=3), _rand(1, 1, D, seed=4), _rand(1, 1, D, seed=5)
+    (v1[0, 0] if new else v[0, 5, 0])[3] = float("nan")
+    cache.fill(k, v)
+    out = cache.step(q, k1, v1)
+    assert out[..., :32].isnan().all()
+    assert torch.isfinite(out[..., 32:]).all()
