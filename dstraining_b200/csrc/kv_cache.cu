@@ -18,9 +18,10 @@
 //   * the up to 8 query heads that share a key head are the rows of
 //     mma.m16n8k16 (one query row per head: a 128-row tcgen05 tile would be
 //     empty for the most part, and at 8 rows the instruction is not the bound);
-//     4-bit codes become bf16 operands with one bit operation per pair (128 +
-//     code is exact in bf16), the steps and least values are applied to the fp32
-//     scores and to the probabilities, never to rounded keys or values;
+//     4-bit codes become bf16 operands with one bit operation per pair (128 + code
+//     is exact in bf16) and for values a subtraction (code - 8 is too), the steps
+//     and least values are applied to the fp32 scores and to the probabilities,
+//     never to rounded keys or values;
 //   * probabilities enter the second product as the sum of two bf16 numbers in
 //     the unused rows 8..15 (relative error 2^-17), so the result carries the
 //     precision of fp32 probabilities.
@@ -111,6 +112,8 @@ __device__ __forceinline__ Quant8 quantize8(const float (&x)[8]) {
 
 __device__ __forceinline__ float param_step(uint32_t p) { return __uint_as_float(p << 16); }
 __device__ __forceinline__ float param_low(uint32_t p) { return __uint_as_float(p & 0xffff0000u); }
+// What code 8 stands for.
+__device__ __forceinline__ float param_middle(uint32_t p) { return fmaf(8.f, param_step(p), param_low(p)); }
 
 // Layout of a packed row of DP channels, NG = DP / 32 groups.
 //   keys:   word (t, g), t = 0..3, at 4 (t NG + g): the channels g*32 + t*8 + c;
@@ -356,9 +359,16 @@ struct StepArgs {
 //
 // Packed rows: the scores are computed transposed (a row of the mma is a key, so
 // all 16 rows are used and the codes of a key go in as they come), so a thread's
-// m and l are those of the query rows 2t, 2t + 1, over its keys n, n + 8. The codes
-// enter as 128 + code, and a value has its group's least value: both make a term
-// that is the same for all channels of a group, sum over keys of p low - 128 p step.
+// m and l are those of the query rows 2t, 2t + 1, over its keys n, n + 8. The codes of
+// keys enter as 128 + code, those of values as code - 8; what code 8 stands for makes a
+// term that is the same for all channels of a group, the sum over keys of
+// p (low + 8 step), in each group's own fp32 sum (one that the groups share would spread
+// a group that stands for NaN over all). Values have to lie around zero: each
+// accumulation of the mma cuts the sum's low bits, so a sum over thousands of keys that a
+// bias makes larger than the result loses the result's. With 128 + code, and the bias
+// taken back by a sum of its own, the error grew with the keys a warp adds up, to 11% at
+// 8192. A score is a sum of 4 or 8 products, where the bias costs nothing that shows (the
+// same error to 6 digits, also for queries 16 times as large) and the subtraction 3%.
 template <int DP, int ROWS>
 struct State {
   static constexpr int NG = DP / 32;
@@ -368,12 +378,11 @@ struct State {
   static constexpr int kTiles = ROWS == kPackedGroups ? 4 : DP / 8;
   float m[kHeads], l[kHeads];
   float o[kTiles][4];  // [tile]: 0, 1 high parts, 2, 3 low parts of the probabilities
-  float c[4];          // packed groups: -128 sum p step of the row's group
-  float low[ROWS == kPackedHeads ? NG : 1][2];  // sum p low (packed heads: p (low - 128 step)) of query row 2t, 2t + 1
+  float low[ROWS == kPackedHeads ? NG : 1][2];  // sum p (low + 8 step) of (group,) query row 2t, 2t + 1
 };
 
-// The query rows as mma operands. Packed: also -128 times their sums over groups
-// for the query rows 2t, 2t + 1, and those sums to be multiplied with the least
+// The query rows as mma operands. Packed: also -128 times their sums over groups for
+// the query rows 2t, 2t + 1 (packed groups: once), and those sums to be multiplied with the least
 // values of a key (packed heads: as three bf16 parts).
 template <int DP, int ROWS>
 struct Query {
@@ -480,13 +489,14 @@ __device__ __forceinline__ void attend_bf16(State<DP, kBf16Heads>& st, const Que
 }
 
 // Codes i and i + 4 of a word as a bf16 pair of 128 + code: a shift, and one
-// three-input operation for mask and exponent (with both constants in registers;
-// as immediates they took one each).
+// three-input operation for mask and exponent (with both constants in registers; as
+// immediates they took one each). Centred: code - 8, by a subtraction (exact).
 struct Codes {
-  uint32_t mask, exponent;
+  uint32_t mask, exponent, middle;
   __device__ __forceinline__ Codes() {
     asm volatile("mov.u32 %0, 0x000f000f;" : "=r"(mask));
     asm volatile("mov.u32 %0, 0x43004300;" : "=r"(exponent));
+    asm volatile("mov.u32 %0, 0x43084308;" : "=r"(middle));
   }
   __device__ __forceinline__ uint32_t first(uint32_t w) const {
     uint32_t r;
@@ -496,6 +506,13 @@ struct Codes {
   __device__ __forceinline__ void all(uint32_t w, uint32_t (&pair)[4]) const {
 #pragma unroll
     for (int i = 0; i < 4; ++i) pair[i] = first(w >> (4 * i));
+  }
+  __device__ __forceinline__ void centred(uint32_t w, uint32_t (&pair)[4]) const {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      pair[i] = first(w >> (4 * i));
+      asm("sub.bf16x2 %0, %0, %1;" : "+r"(pair[i]) : "r"(middle));
+    }
   }
 };
 
@@ -620,8 +637,6 @@ __device__ __forceinline__ void attend_packed(State<DP, ROWS>& st, const Query<D
 #pragma unroll
       for (int j = 0; j < 4; ++j) st.o[i][j] *= cn;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) st.c[j] *= cn;
-#pragma unroll
     for (int g = 0; g < (ROWS == kPackedHeads ? NG : 1); ++g)
 #pragma unroll
       for (int e = 0; e < 2; ++e) st.low[g][e] *= c[NH == 2 ? e : 0];
@@ -661,8 +676,8 @@ __device__ __forceinline__ void attend_packed(State<DP, ROWS>& st, const Query<D
       const uint32_t lo = __byte_perm(w[0][g >> 1], w[1][g >> 1], (g & 1) ? 0x7632 : 0x5410);
       const uint32_t hi = __byte_perm(w[2][g >> 1], w[3][g >> 1], (g & 1) ? 0x7632 : 0x5410);
       uint32_t x[4], y[4];
-      codes.all(lo, x);
-      codes.all(hi, y);
+      codes.centred(lo, x);
+      codes.centred(hi, y);
 #pragma unroll
       for (int j = 0; j < 4; ++j) mma16816(st.o[tile0 + j], a0, a1, a2, a3, x[j], y[j]);
     };
@@ -673,13 +688,11 @@ __device__ __forceinline__ void attend_packed(State<DP, ROWS>& st, const Query<D
         uint2 x = *reinterpret_cast<const uint2*>(par + k * 8 * NG + g0);
         if (masked && !on[k]) x = make_uint2(0u, 0u);
         const float p = s[u][k][0];
-        st.low[0][0] = fmaf(p, param_low(x.x), st.low[0][0]);
-        st.low[0][1] = fmaf(p, param_low(x.y), st.low[0][1]);
+        st.low[0][0] = fmaf(p, param_middle(x.x), st.low[0][0]);
+        st.low[0][1] = fmaf(p, param_middle(x.y), st.low[0][1]);
         split2(p * param_step(x.x), p * param_step(x.y), hi[k], lo[k]);
       }
       const uint32_t a0 = transpose8(hi[0]), a1 = transpose8(lo[0]), a2 = transpose8(hi[1]), a3 = transpose8(lo[1]);
-      constexpr uint32_t kMinus128 = 0xc300c300u;
-      mma16816(st.c, a0, a1, a2, a3, kMinus128, kMinus128);
 #pragma unroll
       for (int g = 0; g < NG; ++g) {  // into the rows of group g alone: one set of sums for all
         const bool mine = (n & (NG - 1)) == g;
@@ -693,11 +706,9 @@ __device__ __forceinline__ void attend_packed(State<DP, ROWS>& st, const Query<D
         for (int k = 0; k < 2; ++k) {
           uint32_t x = par[k * 8 * NG + g];
           if (masked && !on[k]) x = 0u;
-          // the group's own sum takes the bias back: one that the groups share would spread
-          // a group that stands for NaN over all of them
-          const float step = param_step(x), base = fmaf(-128.f, step, param_low(x));
+          const float step = param_step(x);
 #pragma unroll
-          for (int e = 0; e < 2; ++e) st.low[g][e] = fmaf(s[u][k][e], base, st.low[g][e]);
+          for (int e = 0; e < 2; ++e) st.low[g][e] = fmaf(s[u][k][e], param_middle(x), st.low[g][e]);
           split2(s[u][k][0] * step, s[u][k][1] * step, hi[k], lo[k]);
         }
         const uint32_t a0 = transpose8(hi[0]), a1 = transpose8(lo[0]), a2 = transpose8(hi[1]), a3 = transpose8(lo[1]);
@@ -857,8 +868,6 @@ __global__ void __launch_bounds__(kThreads, StepCfg<DP, ROWS>::kCtas)
   for (int i = 0; i < State<DP, ROWS>::kTiles; ++i)
 #pragma unroll
     for (int j = 0; j < 4; ++j) st.o[i][j] = 0.f;
-#pragma unroll
-  for (int j = 0; j < 4; ++j) st.c[j] = 0.f;
 
   // The new token: its row into the cache (once) and, laid out as a tile of one
   // key, into this warp's result.
@@ -961,7 +970,7 @@ __global__ void __launch_bounds__(kThreads, StepCfg<DP, ROWS>::kCtas)
 #pragma unroll
       for (int g = 0; g < NG; ++g) add[g] = to_row(over_keys(st.low[g][0]), over_keys(st.low[g][1]));
     } else {
-      add[0] = to_row(over_keys(st.low[0][0]), over_keys(st.low[0][1])) + st.c[0] + st.c[2];
+      add[0] = to_row(over_keys(st.low[0][0]), over_keys(st.low[0][1]));
     }
   }
   __syncthreads();  // every ring has been read

@@ -307,3 +307,25 @@ def test_a_nan_stays_in_its_group_however_many_heads_share_it(G, D, new):
     out = cache.step(q, k1, v1)
     assert out[..., :32].isnan().all()
     assert torch.isfinite(out[..., 32:]).all()
+
+
+@pytest.mark.parametrize("G", [1, 8])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("bits", [16, 4])
+def test_one_cta_adds_up_a_long_cache(bits, D, G):
+    """More (sequence, key head) pairs than CTAs fit on the GPU: each CTA holds a whole cache, a warp adds up 8192
+    keys, and the error is still that of rounding the result. One set of rows serves all key heads."""
+    from dstraining_b200.ops.kv_cache import WindowCache
+
+    Hk, W, S = 608, 32764, 4  # 4 CTAs an SM: 592
+    T = W + S - 2
+    cache = WindowCache(1, Hk, D, W, S, bits=bits, device="cuda")
+    k, v = _rand(1, T, 1, D, seed=1), _rand(1, T, 1, D, seed=2)
+    cache.fill(k.expand(-1, -1, Hk, -1), v.expand(-1, -1, Hk, -1))
+    q, k1, v1 = _rand(1, Hk * G, D, seed=3), _rand(1, 1, D, seed=4), _rand(1, 1, D, seed=5)
+    out = cache.step(q, k1.expand(-1, Hk, -1), v1.expand(-1, Hk, -1))
+    keys, values = (torch.cat([_stands_for(x[0, :, 0], bits), _stands_for(y[0], bits)]).double()
+                    for x, y in ((k, k1), (v, v1)))
+    some = torch.arange(0, Hk * G, G * Hk // 304, device="cuda")
+    want = torch.softmax(q[0, some].double() @ keys.T * D**-0.5, dim=-1) @ values
+    assert ((out[0, some].double() - want).norm() / want.norm()).item() < 1.1 * U
