@@ -331,8 +331,10 @@ struct StepCfg {
   // the new token's row, laid out like a stage of 16 keys
   static constexpr int kNew = 2 * 16 * (kRowBytes + kParamBytes);
   static constexpr int kJoin = kWarps * kRows * (DP + 2) * 4;  // over the ring at the end
+  static constexpr int kSumStages = 256 / KT;  // packed: the mma sums go to fp32 sums after so many
+  static constexpr int kSums = kPacked ? kThreads * (ROWS == kPackedGroups ? 4 : DP / 8) * 2 * 4 : 0;
   static constexpr int kMaxSplits = kRingBytes / (4 * kRows) - 1;  // their weights too
-  static constexpr int kSmem = (kRingBytes > kJoin ? kRingBytes : kJoin) + kNew + kWarps * kStages * 8 + 16 + 1024;
+  static constexpr int kSmem = (kRingBytes > kJoin ? kRingBytes : kJoin) + kNew + kSums + kWarps * kStages * 8 + 16 + 1024;
   static constexpr int kCtas = !kPacked ? 2 : ROWS == kPackedGroups ? 4 : DP == 64 ? 4 : 3;  // per SM
   static constexpr int kSub = ROWS == kPackedHeads ? 1 : KT % 32 == 0 ? 2 : 1;  // subtiles of 16 keys at a time
 };
@@ -367,7 +369,7 @@ struct StepArgs {
 // accumulation of the mma cuts the sum's low bits, so a sum over thousands of keys that a
 // bias makes larger than the result loses the result's. With 128 + code, and the bias
 // taken back by a sum of its own, the error grew with the keys a warp adds up, to 11% at
-// 8192. A score is a sum of 4 or 8 products, where the bias costs nothing that shows (the
+// 8192. For the same reason the sums go on to fp32 sums every 256 keys. A score is a sum of 4 or 8 products, where the bias costs nothing that shows (the
 // same error to 6 digits, also for queries 16 times as large) and the subtraction 3%.
 template <int DP, int ROWS>
 struct State {
@@ -718,6 +720,49 @@ __device__ __forceinline__ void attend_packed(State<DP, ROWS>& st, const Query<D
   }
 }
 
+// The output sums so far into fp32 sums in shared memory (first: nothing is there yet),
+// or at the end those added to what the mma holds; `m` are the maxima they go by.
+// Rounded to nearest, a few hundred keys at a time, they do not lose what the mma cuts
+// off: with a constant large channel in a group, whose other codes are far from the
+// middle, 8192 keys in one mma sum cost the other channels 1%.
+template <int DP, int ROWS>
+__device__ __forceinline__ float sums_factor(const State<DP, ROWS>& st, float (&m)[State<DP, ROWS>::kHeads]) {
+  constexpr int NH = State<DP, ROWS>::kHeads;
+  const int n = (threadIdx.x & 31) >> 2;
+  float c[NH];
+#pragma unroll
+  for (int e = 0; e < NH; ++e) {
+    c[e] = m[e] == st.m[e] ? 1.f : exp2f(m[e] - st.m[e]);
+    m[e] = st.m[e];
+  }
+  // the factor of output row n lies with the threads that hold column n
+  const float even = __shfl_sync(0xffffffff, c[0], n >> 1), odd = __shfl_sync(0xffffffff, c[NH - 1], n >> 1);
+  return (n & 1) ? odd : even;
+}
+
+template <int DP, int ROWS>
+__device__ __forceinline__ void put_sums(State<DP, ROWS>& st, float* sums, float (&m)[State<DP, ROWS>::kHeads], bool first) {
+  const float c = sums_factor<DP, ROWS>(st, m);
+#pragma unroll
+  for (int i = 0; i < State<DP, ROWS>::kTiles; ++i)
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      float* x = sums + (2 * i + j) * kThreads;
+      const float now = st.o[i][j] + st.o[i][j + 2];
+      *x = first ? now : fmaf(*x, c, now);
+      st.o[i][j] = st.o[i][j + 2] = 0.f;
+    }
+}
+
+template <int DP, int ROWS>
+__device__ __forceinline__ void add_sums(State<DP, ROWS>& st, const float* sums, float (&m)[State<DP, ROWS>::kHeads]) {
+  const float c = sums_factor<DP, ROWS>(st, m);
+#pragma unroll
+  for (int i = 0; i < State<DP, ROWS>::kTiles; ++i)
+#pragma unroll
+    for (int j = 0; j < 2; ++j) st.o[i][j] = fmaf(sums[(2 * i + j) * kThreads], c, st.o[i][j]);
+}
+
 template <int DP, int ROWS, int NS>
 __device__ __forceinline__ void attend(State<DP, ROWS>& st, const Query<DP, ROWS>& q, const uint8_t* sk,
                                        const uint8_t* sv, const uint32_t* pk, const uint32_t* pv, int tile_rows,
@@ -742,7 +787,8 @@ __global__ void __launch_bounds__(kThreads, StepCfg<DP, ROWS>::kCtas)
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* fresh = smem + (C::kRingBytes > C::kJoin ? C::kRingBytes : C::kJoin);
-  uint64_t* bars = reinterpret_cast<uint64_t*>(fresh + C::kNew);
+  float* sums = reinterpret_cast<float*>(fresh + C::kNew) + threadIdx.x;  // this thread's, kThreads apart
+  uint64_t* bars = reinterpret_cast<uint64_t*>(fresh + C::kNew + C::kSums);
   int* last_flag = reinterpret_cast<int*>(bars + kWarps * ST);
 
   const int split = blockIdx.x, b = blockIdx.z;
@@ -915,6 +961,9 @@ __global__ void __launch_bounds__(kThreads, StepCfg<DP, ROWS>::kCtas)
   }
 
   bool ok = true;
+  float m_sums[State<DP, ROWS>::kHeads];  // the maxima that the sums in shared memory go by
+#pragma unroll
+  for (int e = 0; e < State<DP, ROWS>::kHeads; ++e) m_sums[e] = -INFINITY;
   for (int i = 0; i < mine && ok; ++i) {
     const int stage = i % ST;
     ok = __all_sync(0xffffffff, mbar_wait(&full[stage], (i / ST) & 1, a.status, kTimeoutTmaFull));
@@ -939,7 +988,11 @@ __global__ void __launch_bounds__(kThreads, StepCfg<DP, ROWS>::kCtas)
     __syncwarp();
     if (lane == 0 && loaded < mine) load(loaded++);
     __syncwarp();
+    if constexpr (C::kPacked)
+      if ((i + 1) % C::kSumStages == 0) put_sums<DP, ROWS>(st, sums, m_sums, i + 1 == C::kSumStages);
   }
+  if constexpr (C::kPacked)
+    if (ok && mine >= C::kSumStages) add_sums<DP, ROWS>(st, sums, m_sums);
   if (!ok && lane == 0)  // a wait expired: no copy may land after the CTA is gone
     for (int i = max(0, loaded - ST); i < loaded; ++i) mbar_wait(&full[i % ST], (i / ST) & 1, a.status, kTimeoutTmaFull);
 

@@ -329,3 +329,26 @@ def test_one_cta_adds_up_a_long_cache(bits, D, G):
     some = torch.arange(0, Hk * G, G * Hk // 304, device="cuda")
     want = torch.softmax(q[0, some].double() @ keys.T * D**-0.5, dim=-1) @ values
     assert ((out[0, some].double() - want).norm() / want.norm()).item() < 1.1 * U
+
+
+@pytest.mark.parametrize("G", [1, 8])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("large", [8.0, 30.0])
+def test_one_cta_adds_up_values_beside_a_large_channel(large, D, G):
+    """One channel of each group is large and of one sign, so the others' codes are far from the middle: their sums
+    cancel, and still are as good as their rounding."""
+    from dstraining_b200.ops.kv_cache import WindowCache
+
+    Hk, T = 608, 32766
+    k, v = _rand(1, T, 1, D, seed=1), _rand(1, T, 1, D, seed=2)
+    q, k1, v1 = _rand(1, Hk * G, D, seed=3), _rand(1, 1, D, seed=4), _rand(1, 1, D, seed=5)
+    for x in (v, v1):
+        x[..., 7::32] = large + x[..., 7::32].abs()
+    cache = WindowCache(1, Hk, D, T + 2, 0, bits=4, device="cuda")
+    cache.fill(k.expand(-1, -1, Hk, -1), v.expand(-1, -1, Hk, -1))
+    out = cache.step(q, k1.expand(-1, Hk, -1), v1.expand(-1, Hk, -1))
+    keys, values = (torch.cat([_stands_for(x[0, :, 0], 4), _stands_for(y[0], 4)]).double() for x, y in ((k, k1), (v, v1)))
+    some = torch.arange(0, Hk * G, G * Hk // 304, device="cuda")
+    want = torch.softmax(q[0, some].double() @ keys.T * D**-0.5, dim=-1) @ values
+    for part in (slice(7, None, 32), slice(8, None, 32), slice(31, None, 32)):
+        assert ((out[0, some, part].double() - want[:, part]).norm() / want[:, part].norm()).item() < 1.2 * U
