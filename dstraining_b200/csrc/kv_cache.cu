@@ -52,6 +52,7 @@ namespace kv_cache {
 constexpr int kWarps = 4;
 constexpr int kThreads = 32 * kWarps;
 constexpr int kRows = 8;  // query heads per CTA
+constexpr int kMostCtas = 4;  // CTAs per SM of any step kernel
 
 // ------------------------------------------------------------ row formats
 // 8 channels of a row as one lane holds them.
@@ -336,6 +337,7 @@ struct StepCfg {
   static constexpr int kMaxSplits = kRingBytes / (4 * kRows) - 1;  // their weights too
   static constexpr int kSmem = (kRingBytes > kJoin ? kRingBytes : kJoin) + kNew + kSums + kWarps * kStages * 8 + 16 + 1024;
   static constexpr int kCtas = !kPacked ? 2 : ROWS == kPackedGroups ? 4 : DP == 64 ? 4 : 3;  // per SM
+  static_assert(kCtas <= kMostCtas, "the arrival counters are too few");
   static constexpr int kSub = ROWS == kPackedHeads ? 1 : KT % 32 == 0 ? 2 : 1;  // subtiles of 16 keys at a time
 };
 
@@ -348,7 +350,7 @@ struct StepArgs {
   __nv_bfloat16* out;      // [B, H, D]
   float *stored_k, *stored_v;  // optional [B, Hk, D]: what the new row stands for
   float* partial;          // [B * Hk * chunks][splits][kRows][DP + 2]
-  int* arrived;            // [B * Hk * chunks], 0 between launches
+  int* arrived;            // [B * Hk * chunks] where splits > 1, 0 between launches
   Ring ring;
   int slots, Hk, G, D, chunks, splits;
   float scale_log2;
@@ -1170,6 +1172,10 @@ class KVCache {
       store_[i] = {static_cast<uint8_t*>(rows_[i].data_ptr()),
                    bits == 4 ? static_cast<uint32_t*>(params_[i].data_ptr()) : nullptr};
     }
+    // Not with the first step: that may be one that a graph captures, and the counters
+    // have to be 0 for steps outside of it too. Units that share the GPU among more than
+    // one CTA each are at most half as many as fit on it.
+    arrived_ = at::zeros({kMostCtas * num_sms() / 2}, options.dtype(at::kInt));
     dispatch([&](auto dp, auto bits_c) {
       if constexpr (bits_c() == 16) {
         const uint64_t n = static_cast<uint64_t>(B_) * Hk_ * alloc;
@@ -1259,7 +1265,7 @@ class KVCache {
       a.stored_v = result[2].data_ptr<float>();
     }
     a.partial = work.partial.data_ptr<float>();
-    a.arrived = work.arrived.data_ptr<int>();
+    a.arrived = arrived_.data_ptr<int>();
     a.ring = ring_;
     a.slots = static_cast<int>(slots_), a.Hk = static_cast<int>(Hk_), a.G = static_cast<int>(G);
     a.D = static_cast<int>(D_), a.chunks = static_cast<int>(chunks), a.splits = work.splits;
@@ -1285,9 +1291,9 @@ class KVCache {
   const at::Tensor& params(int i) const { return params_[i]; }
 
  private:
-  struct Work {  // joining the CTAs that share a cache; the counters are 0 between launches
+  struct Work {  // joining the CTAs that share a cache
     int splits;
-    at::Tensor partial, arrived;
+    at::Tensor partial;
   };
 
   template <typename F>
@@ -1329,8 +1335,7 @@ class KVCache {
       const int64_t most = (slots_ + kWarps * C::KT - 1) / (kWarps * C::KT);
       splits = std::min({most, std::max<int64_t>(1, C::kCtas * num_sms() / units), int64_t(C::kMaxSplits)});
     });
-    Work w = {static_cast<int>(splits), at::empty({units * splits * kRows * (DP_ + 2)}, pos_.options().dtype(at::kFloat)),
-              at::zeros({units}, pos_.options().dtype(at::kInt))};
+    Work w = {static_cast<int>(splits), at::empty({units * splits * kRows * (DP_ + 2)}, pos_.options().dtype(at::kFloat))};
     return work_.emplace(chunks, std::move(w)).first->second;
   }
 
@@ -1349,6 +1354,7 @@ class KVCache {
   int64_t B_, Hk_, D_, slots_, DP_;
   int bits_;
   at::Tensor pos_, rows_[2], params_[2];
+  at::Tensor arrived_;  // per unit of a step, 0 between launches
   Store store_[2];
   Ring ring_;
   CUtensorMap map_[2] = {};

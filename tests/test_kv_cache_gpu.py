@@ -352,3 +352,38 @@ def test_one_cta_adds_up_values_beside_a_large_channel(large, D, G):
     want = torch.softmax(q[0, some].double() @ keys.T * D**-0.5, dim=-1) @ values
     for part in (slice(7, None, 32), slice(8, None, 32), slice(31, None, 32)):
         assert ((out[0, some, part].double() - want[:, part]).norm() / want[:, part].norm()).item() < 1.2 * U
+
+
+@pytest.mark.parametrize("bits", [16, 4])
+def test_first_step_under_capture(bits):
+    """A cache whose first step is captured: steps outside the graph are right before and after its replays."""
+    from dstraining_b200.ops.kv_cache import WindowCache
+
+    H, D = 2, 64
+    k, v = _rand(1, 3000, H, D, seed=1), _rand(1, 3000, H, D, seed=2)
+    q, k1, v1 = (_rand(1, H, D, seed=i) for i in (3, 4, 5))
+    pos = torch.tensor([3000], device="cuda")
+
+    def make():
+        cache = WindowCache(1, H, D, 4000, 4, bits=bits, device="cuda")
+        cache.fill(k, v)
+        return cache
+
+    want = make().step(q, k1, v1, pos)
+    cache = make()
+    # the graphs' memory holds sevens
+    pool, g0 = torch.cuda.graph_pool_handle(), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g0, pool=pool):
+        dirt = [torch.full((2**17,), 7, dtype=torch.int32, device="cuda") for _ in range(16)]
+    g0.replay()
+    del dirt
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, pool=pool):
+        captured = cache.step(q, k1, v1, pos)
+    for _ in range(2):
+        got = torch.full_like(want, float("nan"))  # where the next result may land
+        del got
+        assert torch.equal(cache.step(q, k1, v1, pos), want)
+    g.replay()
+    assert torch.equal(captured, want)
+    assert torch.equal(cache.step(q, k1, v1, pos), want)
