@@ -42,6 +42,7 @@
 #include <algorithm>
 #include <map>
 #include <string>
+#include <utility>
 
 #include "common.h"
 #include "ptx.cuh"
@@ -1325,8 +1326,10 @@ class KVCache {
   // How many CTAs share the slots of one (sequence, key head): as many as fit on the
   // GPU at once (a few more would run after all others: 57 us against 54 for 16
   // sequences of 2 key heads), each with at least one tile per warp.
+  // It depends on the number of query heads alone, so by no earlier call's.
   const Work& work_for(int64_t chunks, Rows rows) {
-    auto it = work_.find(chunks);
+    const auto key = std::make_pair(chunks, rows);
+    auto it = work_.find(key);
     if (it != work_.end()) return it->second;
     const int64_t units = B_ * Hk_ * chunks;
     int64_t splits = 1;
@@ -1336,7 +1339,7 @@ class KVCache {
       splits = std::min({most, std::max<int64_t>(1, C::kCtas * num_sms() / units), int64_t(C::kMaxSplits)});
     });
     Work w = {static_cast<int>(splits), at::empty({units * splits * kRows * (DP_ + 2)}, pos_.options().dtype(at::kFloat))};
-    return work_.emplace(chunks, std::move(w)).first->second;
+    return work_.emplace(key, std::move(w)).first->second;
   }
 
   void check_rows(const at::Tensor& x, std::initializer_list<int64_t> sizes, const char* name) const {
@@ -1358,7 +1361,7 @@ class KVCache {
   Store store_[2];
   Ring ring_;
   CUtensorMap map_[2] = {};
-  std::map<int64_t, Work> work_;
+  std::map<std::pair<int64_t, Rows>, Work> work_;  // by chunks and row form
 };
 
 }  // namespace kv_cache

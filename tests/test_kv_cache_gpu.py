@@ -387,3 +387,24 @@ def test_first_step_under_capture(bits):
     g.replay()
     assert torch.equal(captured, want)
     assert torch.equal(cache.step(q, k1, v1, pos), want)
+
+
+@pytest.mark.parametrize("D,G1,G2", [(128, 2, 8), (64, 4, 8)])
+def test_steps_of_one_cache_do_not_depend_on_earlier_ones(D, G1, G2):
+    """Calls with other numbers of query heads leave no trace: the same bits as from a cache of its own."""
+    from dstraining_b200.ops.kv_cache import WindowCache
+
+    B, n = 33, 3000
+    k, v = _rand(B, n, 1, D, seed=1), _rand(B, n, 1, D, seed=2)
+    k1, v1 = _rand(B, 1, D, seed=4), _rand(B, 1, D, seed=5)
+    pos = torch.full((B,), n, device="cuda")
+
+    def make():
+        cache = WindowCache(B, 1, D, n + 100, 0, bits=4, device="cuda")
+        cache.fill(k, v)
+        return cache
+
+    used = make()
+    for G in (G1, G2, G1):
+        q = _rand(B, G, D, seed=6 + G)
+        assert torch.equal(used.step(q, k1, v1, pos), make().step(q, k1, v1, pos))
