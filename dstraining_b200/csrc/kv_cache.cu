@@ -187,6 +187,12 @@ struct Ring {
   __device__ __forceinline__ int64_t slot(int64_t p) const { return p < S ? p : S + (p - S) % W; }
 };
 
+struct Positions {  // int64, one per sequence
+  int64_t* p;
+  int64_t stride;
+  __device__ __forceinline__ int64_t& operator[](int b) const { return p[b * stride]; }
+};
+
 struct View {  // k or v rows: element strides, unit inner stride
   const __nv_bfloat16* p;
   int64_t b, h, t;
@@ -202,14 +208,14 @@ __device__ __forceinline__ uint4 load8(const __nv_bfloat16* row, int i, int D) {
 // of the last window.
 template <int DP, int BITS>
 __global__ void __launch_bounds__(256)
-    fill_kernel(const View k, const View v, const int64_t* __restrict__ lengths, int64_t* __restrict__ pos, Store ks,
-                Store vs, const Ring ring, int T, int rows, int Hk, int D, int* status) {
+    fill_kernel(const View k, const View v, const Positions lengths, const Positions pos, Store ks, Store vs,
+                const Ring ring, int T, int rows, int Hk, int D, int* status) {
   constexpr int L = DP / 8;
   const int64_t r = (static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x) / L;
   const int i = threadIdx.x % L;
   const int b = blockIdx.z, hk = blockIdx.y >> 1;
   const bool value = blockIdx.y & 1;
-  int64_t len = lengths ? lengths[b] : T;
+  int64_t len = lengths.p ? lengths[b] : T;
   if (len < 0 || len > T) {
     if (threadIdx.x == 0) record_status(status, kBadArgument);
     len = len < 0 ? 0 : T;
@@ -243,8 +249,8 @@ __global__ void __launch_bounds__(256)
 // The held rows in slot order (0 where no token is): bf16, or fp32 for 4 bits.
 template <int DP, int BITS>
 __global__ void __launch_bounds__(256)
-    read_kernel(const Store ks, const Store vs, const int64_t* __restrict__ pos, void* __restrict__ ko,
-                void* __restrict__ vo, const Ring ring, int slots, int Hk, int D) {
+    read_kernel(const Store ks, const Store vs, const Positions pos, void* __restrict__ ko, void* __restrict__ vo,
+                const Ring ring, int slots, int Hk, int D) {
   constexpr int L = DP / 8;
   const int64_t r = (static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x) / L;
   const int i = threadIdx.x % L;
@@ -346,7 +352,7 @@ struct StepArgs {
   const __nv_bfloat16* q;
   int64_t q_b, q_h;
   View k, v;  // the new token's rows
-  const int64_t* pos;
+  Positions pos;
   Store ks, vs;
   __nv_bfloat16* out;      // [B, H, D]
   float *stored_k, *stored_v;  // optional [B, Hk, D]: what the new row stands for
@@ -1207,8 +1213,8 @@ class KVCache {
       const dim3 grid(static_cast<unsigned>((static_cast<int64_t>(rows) * (dp() / 8) + 255) / 256),
                       static_cast<unsigned>(2 * Hk_), static_cast<unsigned>(B_));
       fill_kernel<dp(), bits()><<<grid, 256, 0, at::cuda::getCurrentCUDAStream()>>>(
-          kv, vv, lengths ? lengths->data_ptr<int64_t>() : nullptr, pos_.data_ptr<int64_t>(), store_[0], store_[1],
-          ring_, static_cast<int>(T), rows, static_cast<int>(Hk_), static_cast<int>(D_), status_ptr());
+          kv, vv, lengths ? positions(*lengths) : Positions{nullptr, 0}, positions(pos_), store_[0], store_[1], ring_,
+          static_cast<int>(T), rows, static_cast<int>(Hk_), static_cast<int>(D_), status_ptr());
     });
     C10_CUDA_KERNEL_LAUNCH_CHECK();
     debug_check("kv_cache fill");
@@ -1223,7 +1229,7 @@ class KVCache {
       const dim3 grid(static_cast<unsigned>((slots_ * (dp() / 8) + 255) / 256), static_cast<unsigned>(2 * Hk_),
                       static_cast<unsigned>(B_));
       read_kernel<dp(), bits()><<<grid, 256, 0, at::cuda::getCurrentCUDAStream()>>>(
-          store_[0], store_[1], pos_.data_ptr<int64_t>(), k.data_ptr(), v.data_ptr(), ring_, static_cast<int>(slots_),
+          store_[0], store_[1], positions(pos_), k.data_ptr(), v.data_ptr(), ring_, static_cast<int>(slots_),
           static_cast<int>(Hk_), static_cast<int>(D_));
     });
     C10_CUDA_KERNEL_LAUNCH_CHECK();
@@ -1256,7 +1262,7 @@ class KVCache {
     a.q_b = q.stride(0), a.q_h = q.stride(1);
     a.k = {static_cast<const __nv_bfloat16*>(k.data_ptr()), k.stride(0), k.stride(1), 0};
     a.v = {static_cast<const __nv_bfloat16*>(v.data_ptr()), v.stride(0), v.stride(1), 0};
-    a.pos = pos.data_ptr<int64_t>();
+    a.pos = positions(pos);
     a.ks = store_[0], a.vs = store_[1];
     a.out = static_cast<__nv_bfloat16*>(out.data_ptr());
     a.stored_k = a.stored_v = nullptr;
@@ -1350,9 +1356,11 @@ class KVCache {
 
   void check_positions(const at::Tensor& x, const char* name) const {
     TORCH_CHECK_VALUE(x.is_cuda() && (!pos_.defined() || x.device() == pos_.device()) && x.scalar_type() == at::kLong &&
-                          x.is_contiguous() && x.dim() == 1 && x.size(0) == B_,
-                      name, " must be a contiguous int64 tensor [", std::to_string(B_), "] on the cache's device");
+                          x.dim() == 1 && x.size(0) == B_,
+                      name, " must be an int64 tensor [", std::to_string(B_), "] on the cache's device");
   }
+
+  static Positions positions(const at::Tensor& x) { return {x.data_ptr<int64_t>(), x.stride(0)}; }
 
   int64_t B_, Hk_, D_, slots_, DP_;
   int bits_;

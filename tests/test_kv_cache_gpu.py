@@ -408,3 +408,24 @@ def test_steps_of_one_cache_do_not_depend_on_earlier_ones(D, G1, G2):
     for G in (G1, G2, G1):
         q = _rand(B, G, D, seed=6 + G)
         assert torch.equal(used.step(q, k1, v1, pos), make().step(q, k1, v1, pos))
+
+
+@pytest.mark.parametrize("bits", [16, 4])
+def test_positions_of_any_stride(bits):
+    """Positions and lengths as columns of larger tables, also the cache's own."""
+    from dstraining_b200.ops.kv_cache import WindowCache
+
+    table = torch.tensor([[12, 30, -7], [40, 3, -7], [41, 0, -7]], device="cuda")
+    own = torch.zeros(3, 2, dtype=torch.int64, device="cuda")
+    k, v = _rand(3, 40, 2, 64, seed=1), _rand(3, 40, 2, 64, seed=2)
+    q, k1, v1 = _rand(3, 4, 64, seed=3), _rand(3, 2, 64, seed=4), _rand(3, 2, 64, seed=5)
+    a = WindowCache(3, 2, 64, 20, 2, bits=bits, device="cuda", pos=own[:, 1])
+    b = WindowCache(3, 2, 64, 20, 2, bits=bits, device="cuda")
+    a.fill(k, v, table[:, 1])
+    b.fill(k, v, table[:, 1].contiguous())
+    assert own.tolist() == [[0, 30], [0, 3], [0, 0]]
+    assert all(torch.equal(x, y) for x, y in zip(a.read(), b.read()))
+    assert torch.equal(a.step(q, k1, v1, table[:, 0]), b.step(q, k1, v1, table[:, 0].contiguous()))
+    assert torch.equal(a.step(q, k1, v1), b.step(q, k1, v1))
+    assert own.tolist() == [[0, 31], [0, 4], [0, 1]] and b.pos.tolist() == [31, 4, 1]
+    assert all(torch.equal(x, y) for x, y in zip(a.read(), b.read()))
