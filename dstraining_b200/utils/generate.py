@@ -8,7 +8,9 @@
 optionally from the ``top_k`` most probable and / or the nucleus of
 probability ``top_p``. With ``device_sampling`` (or ``min_p``) the tokens are
 drawn on the model's device by :func:`~dstraining_b200.ops.sampling.sample_tokens`
-and nothing is copied to the host per token.
+and nothing is copied to the host per token. Logits that leave no token to draw
+(NaN throughout) raise ``RuntimeError``: at their token on the host's path, after
+the last one with ``device_sampling``.
 
 * With ``use_cache=True`` (the default) the prompt is run once and every
   later token costs one row per layer: its key and value are appended to a
@@ -180,6 +182,7 @@ def generate(model: GPT, idx: torch.Tensor, max_new_tokens: int, temperature: fl
     cache = KVCache(model, idx.shape[0], cache_bits) if use_cache else None
     was_training = model.training
     model.eval()
+    broken = None  # whether some row of logits had nothing to draw from, on the device
     try:
         for _ in range(max_new_tokens):
             if cache is None or idx.shape[1] > cfg.block_size:
@@ -192,11 +195,17 @@ def generate(model: GPT, idx: torch.Tensor, max_new_tokens: int, temperature: fl
                 noise = gumbel_noise(*logits.shape, generator.device if generator is not None else logits.device, generator)
                 nxt = sample_tokens(logits, noise.to(logits.device), max(temperature, 0.0), top_k or 0,
                                     1.0 if top_p is None else top_p, min_p or 0.0)[0][:, None]
+                # -1 must not reach the embedding; the error waits for the end, where one copy to the host tells
+                bad = (nxt < 0).any()
+                broken = bad if broken is None else broken | bad
+                nxt = nxt.clamp(min=0)
             else:
                 nxt = _sample(logits, temperature, top_k, generator, top_p)
             idx = torch.cat([idx, nxt.to(idx.dtype)], dim=1)
     finally:
         model.train(was_training)
+    if broken is not None and broken.item():
+        raise RuntimeError("generate: a row of logits is NaN or -inf throughout, there is no token to draw")
     return idx
 
 

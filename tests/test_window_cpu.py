@@ -198,3 +198,22 @@ def test_gumbel_noise_is_standard():
     # mean 0.5772, standard deviation pi / sqrt(6); 5 standard errors of 200000 numbers
     assert abs(g.mean() - 0.57722) < 5 * 1.2825 / math.sqrt(2e5)
     assert abs(g.std() - 1.2825) < 0.02
+
+
+@pytest.mark.parametrize("use_cache", [True, False])
+@pytest.mark.parametrize("tokens", [1, 4])
+@pytest.mark.parametrize("kw", [dict(device_sampling=True), dict(min_p=0.1), dict(device_sampling=True, temperature=0.0)])
+def test_logits_without_a_token_raise(kw, tokens, use_cache):
+    """A model that returns NaN: a clear error, no token of -1 fed back or returned."""
+    m = GPT(GPTConfig(**CFG, attention_window=16), SINGLE, seed=7).eval()
+    seq = torch.randint(0, 300, (2, 30), generator=_gen(2))
+    with torch.no_grad():
+        m.lm_head.weight.fill_(float("nan"))
+    with pytest.raises(RuntimeError, match="no token to draw"):
+        generate(m, seq, tokens, use_cache=use_cache, **kw)
+
+
+def test_nothing_to_generate():
+    m = GPT(GPTConfig(**CFG), SINGLE, seed=7).eval()
+    seq = torch.randint(0, 300, (2, 30), generator=_gen(2))
+    assert torch.equal(generate(m, seq, 0, device_sampling=True), seq)
