@@ -80,14 +80,17 @@ void run_fwd(const Operand& q, const Operand& k, const Operand& v, const Operand
   C10_CUDA_KERNEL_LAUNCH_CHECK();
 }
 
-// Chunks of about a key block's own window, at least 8 blocks of queries.
+// Chunks of about a key block's own window, at least 8 blocks of queries, and no
+// more of them than keep the sums within T rows.
 SinkChunks plan_sinks(const Shape& s) {
-  SinkChunks c = {0, 0, 0, nullptr};
+  SinkChunks c = {0, 0, 0, 0, nullptr};
   const int last_block = (s.T - 1) >> 6;
   for (int k0 = 0; k0 < s.S && (last_window_query(s, k0) >> 6) < last_block; k0 += 128) ++c.blocks;
   if (c.blocks == 0) return c;
-  c.steps = std::max(8, (127 + s.W) / 64 + 1);
-  c.chunks = (last_block - (last_window_query(s, 0) >> 6) + c.steps - 1) / c.steps;
+  c.rows = std::min(s.S, c.blocks * 128);
+  const int far = last_block - (last_window_query(s, 0) >> 6), most = std::max(1, s.T / c.rows - 1);
+  c.steps = std::max({8, (127 + s.W) / 64 + 1, (far + most - 1) / most});
+  c.chunks = (far + c.steps - 1) / c.steps;
   return c;
 }
 
@@ -104,7 +107,7 @@ void run_bwd(__nv_bfloat16* dout, const Operand& q, const Operand& k, const Oper
   SinkChunks sinks = plan_sinks(s);
   at::Tensor partial;
   if (sinks.blocks) {
-    partial = at::empty({B * Hk * sinks.blocks * (1 + sinks.chunks) * 2 * 128 * DP}, f32);
+    partial = at::empty({B * Hk * sinks.rows * (1 + sinks.chunks) * 2 * DP}, f32);
     sinks.partial = partial.data_ptr<float>();
   }
   const CUtensorMap k64 = map_of(k, B, s.T, Hk, s.D, 64), v64 = map_of(v, B, s.T, Hk, s.D, 64);

@@ -64,12 +64,20 @@ struct Operand {  // q, k, v or a gradient: [B, T, heads, D], unit inner stride
 // Sinks are seen by every later query, so their key blocks would walk the whole
 // sequence alone. The queries past the blocks' windows are cut into chunks of
 // `steps` 64-query blocks (per query head), each its own CTA, whose sums for the
-// sink rows are joined in order. Chunk 0 is the block's own window.
+// sink rows are joined in order. Chunk 0 is the block's own window. Of many sinks
+// the blocks are CTAs enough, so rows (1 + chunks) stays within T, or chunks is 1:
+// the sums take no more than twice dK and dV in fp32, whatever S.
 struct SinkChunks {
   int blocks;  // key blocks of 128 that hold sinks and have queries past their window
+  int rows;    // sinks in these blocks
   int chunks;  // CTAs per such block beside its own
   int steps;
-  float* partial;  // [B, Hk, blocks, 1 + chunks, 2, 128, DP]: dK, dV of a chunk
+  float* partial;  // [B, Hk, 1 + chunks, 2, rows, DP]: dK (0) and dV (1) of a chunk
+  template <int DP>
+  __host__ __device__ float* sums(int b, int key_heads, int hk, int chunk, int which, int key) const {
+    const int64_t unit = static_cast<int64_t>(b) * key_heads + hk;
+    return partial + (((unit * (1 + chunks) + chunk) * 2 + which) * rows + key) * DP;
+  }
 };
 
 __host__ __device__ inline int last_window_query(const Shape& s, int k0) {  // of the key block from k0

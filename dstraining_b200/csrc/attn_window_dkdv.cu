@@ -233,10 +233,6 @@ __global__ void __launch_bounds__(DkdvCfg<DP>::kThreads, DkdvCfg<DP>::kCtas)
       const int c0 = group * kShare;
       // sink rows of a cut block are sums of a chunk only: joined over the stored tile later
       const bool to_partial = cut && key < s.S;
-      float* part = cut ? sinks.partial +
-                              ((((static_cast<int64_t>(b) * gridDim.y + hk) * sinks.blocks + kb) * (1 + sinks.chunks) + chunk) *
-                                   2 * 128 + r) * DP
-                        : nullptr;
 #pragma unroll
       for (int ch = 0; ch < kShare / 32; ++ch) {
         const int c = c0 + ch * 32;
@@ -245,7 +241,7 @@ __global__ void __launch_bounds__(DkdvCfg<DP>::kThreads, DkdvCfg<DP>::kCtas)
         for (int which = 0; which < 2; ++which) {
           tmem_ld32_sync((which ? tDV : tDK) + c + lane_off, x);
           if (to_partial) {
-            float4* dst = reinterpret_cast<float4*>(part + which * 128 * DP + c);
+            float4* dst = reinterpret_cast<float4*>(sinks.sums<DP>(b, gridDim.y, hk, chunk, which, key) + c);
 #pragma unroll
             for (int j = 0; j < 8; ++j) dst[j] = make_float4(x[4 * j], x[4 * j + 1], x[4 * j + 2], x[4 * j + 3]);
           }

@@ -45,15 +45,29 @@ __global__ void __launch_bounds__(kThreads, 2)
     const int kb = blockIdx.x - tiles, k0 = kb * 128, rows = min(128, s.S - k0);
     const int first = (last_window_query(s, k0) >> 6) + 1, far = ((s.T - 1) >> 6) - first + 1;
     const int parts = 1 + (far + sinks.steps - 1) / sinks.steps;
-    const float* part =
-        sinks.partial + ((static_cast<int64_t>(b) * (s.H / s.G) + hk) * sinks.blocks + kb) * (1 + sinks.chunks) * 2 * 128 * DP;
-    for (int i = threadIdx.x; i < 2 * rows * DP; i += kThreads) {
-      const int d = i % DP, r = i / DP % rows, which = i / DP / rows;
-      if (d >= s.D) continue;
-      float x = 0.f;
-      for (int c = 0; c < parts; ++c) x += part[(static_cast<int64_t>(c) * 2 + which) * 128 * DP + r * DP + d];
+    constexpr int V = DP / 32;  // channels a lane; a warp takes a row
+    const int c0 = (threadIdx.x & 31) * V;
+    const int64_t step = static_cast<int64_t>(sinks.rows) * 2 * DP;
+    for (int i = threadIdx.x >> 5; i < 2 * rows; i += kThreads / 32) {
+      const int which = i >= rows, r = i - which * rows;
+      const float* part = sinks.sums<DP>(b, s.H / s.G, hk, 0, which, k0 + r) + c0;
+      float x[V] = {};
+#pragma unroll 4
+      for (int c = 0; c < parts; ++c) {
+#pragma unroll
+        for (int j = 0; j < V; j += 2) {
+          const float2 y = *reinterpret_cast<const float2*>(part + c * step + j);
+          x[j] += y.x;
+          x[j + 1] += y.y;
+        }
+      }
       const Operand& g = which ? dv : dk;
-      g.p[b * g.s.b + static_cast<int64_t>(k0 + r) * g.s.t + hk * g.s.h + d] = __float2bfloat16(which ? x : x * s.scale);
+      const float scale = which ? 1.f : s.scale;
+      __nv_bfloat16* out = g.p + b * g.s.b + static_cast<int64_t>(k0 + r) * g.s.t + hk * g.s.h + c0;
+      if (c0 < s.D)
+#pragma unroll
+        for (int j = 0; j < V; j += 2)
+          *reinterpret_cast<uint32_t*>(out + j) = pack_bf16(x[j] * scale, x[j + 1] * scale);
     }
     return;
   }

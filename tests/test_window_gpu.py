@@ -317,3 +317,50 @@ def test_refusals():
         lib.window_attention_qkv(x[0], x[1][:, :7], x[2][:, :7], 4, 0)
     with pytest.raises(RuntimeError, match="window >= 1"):
         lib.window_attention(_rand(1, 8, 3 * 128, seed=0), 2, 64, 0, 0)
+
+
+@pytest.mark.parametrize("T,S", [(4096, 4096), (8192, 8192), (8192, 1500)])
+def test_workspace_stays_linear(T, S):
+    """Many sinks: beside its results the backward pass holds no more than twice dK and dV in fp32 (and the row sums)."""
+    from dstraining_b200.ops.window import window_attention_qkv
+
+    H, D, W = 2, 128, 100
+    x = [_rand(1, T, H, D, seed=i).requires_grad_() for i in range(3)]
+    dout = _rand(1, T, H, D, seed=5)
+    out = window_attention_qkv(*x, W, S)
+    torch.cuda.synchronize()
+    before = torch.cuda.memory_allocated()
+    torch.cuda.reset_peak_memory_stats()
+    grads = torch.autograd.grad(out, x, dout)
+    torch.cuda.synchronize()
+    elements = T * H * D
+    assert torch.cuda.max_memory_allocated() - before <= 3 * 2 * elements + 2 * 2 * 4 * elements + 4 * T * H + 2**16
+    del grads
+
+
+SINK_CHUNKS = [
+    # B, T, H, Hk, D, window, sinks: three or more chunks of far queries a sink block
+    (1, 3000, 2, 1, 128, 64, 5),
+    (1, 2500, 4, 2, 128, 100, 1),
+    (2, 2049, 2, 2, 128, 30, 130),
+    (1, 2700, 3, 1, 64, 64, 260),
+    (1, 4001, 2, 2, 96, 700, 3),
+    (1, 2200, 2, 1, 128, 40, 1100),
+    (1, 1500, 2, 1, 64, 20, 1500),
+]
+
+
+@pytest.mark.parametrize("B,T,H,Hk,D,W,S", SINK_CHUNKS)
+def test_gradients_of_sinks_over_many_chunks(B, T, H, Hk, D, W, S):
+    from dstraining_b200.ops.window import window_attention_qkv
+
+    q, k, v = _rand(B, T, H, D, seed=1), _rand(B, T, Hk, D, seed=2), _rand(B, T, Hk, D, seed=3)
+    dout = _rand(B, T, H, D, seed=4)
+    x = [t.requires_grad_() for t in (q, k, v)]
+    out = window_attention_qkv(*x, W, S)
+    got = (out.detach(), *torch.autograd.grad(out, x, dout))
+    want = _exact(q, k, v, W, S, dout)
+    for name, a, b, tol in zip(("out", "dq", "dk", "dv"), got, want, (2 * U, 4 * U, 4 * U, 2 * U)):
+        assert _err(a, b) < tol, name
+    for name, a, b, tol in (("dk", got[2], want[2], 4 * U), ("dv", got[3], want[3], 2 * U)):  # of the sinks alone
+        assert _err(a[:, :S], b[:, :S]) < tol, name
