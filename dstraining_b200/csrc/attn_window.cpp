@@ -148,6 +148,18 @@ void backward(const at::Tensor& dout, const Operand& q, const Operand& k, const 
 using torch::autograd::AutogradContext;
 using torch::autograd::variable_list;
 
+// The gradients under create_graph: as they are, with a node that refuses to be
+// differentiated. Without one they would count as constants, silently.
+struct FirstOnly : public torch::autograd::Function<FirstOnly> {
+  static variable_list forward(AutogradContext*, at::TensorList gradients, at::TensorList /*of what*/) {
+    return gradients.vec();
+  }
+  static variable_list backward(AutogradContext*, variable_list) {
+    TORCH_CHECK(false, "window attention: no second derivative on CUDA bf16 tensors");
+    return {};
+  }
+};
+
 // Separate q, k, v. The autograd nodes are C++: a Python node costs more host
 // time per call than a short sequence takes on the GPU.
 struct SeparateFn : public torch::autograd::Function<SeparateFn> {
@@ -174,7 +186,12 @@ struct SeparateFn : public torch::autograd::Function<SeparateFn> {
     attn_window::backward(grads[0], operand(q), operand(k), operand(v), out, lse, operand(dq), operand(dk), operand(dv),
                           q.size(0), s);
     debug_check("window_attention backward");
-    return {dq, dk, dv, at::Tensor(), at::Tensor()};
+    variable_list g = {dq, dk, dv};
+    if (at::GradMode::is_enabled()) {
+      const variable_list of = {grads[0], q, k, v};
+      g = FirstOnly::apply(at::TensorList(g), at::TensorList(of));
+    }
+    return {g[0], g[1], g[2], at::Tensor(), at::Tensor()};
   }
 };
 
@@ -205,6 +222,10 @@ struct FusedFn : public torch::autograd::Function<FusedFn> {
     attn_window::backward(grads[0], part_of(qkv, 0, D), part_of(qkv, 1, D), part_of(qkv, 2, D), out, lse,
                           part_of(dqkv, 0, D), part_of(dqkv, 1, D), part_of(dqkv, 2, D), B, s);
     debug_check("window_attention backward");
+    if (at::GradMode::is_enabled()) {
+      const variable_list of = {grads[0], qkv};
+      dqkv = FirstOnly::apply(at::TensorList(dqkv), at::TensorList(of))[0];
+    }
     return {dqkv, at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor()};
   }
 };

@@ -11,7 +11,8 @@ Key ``j`` is visible to query ``i`` iff ``j <= i`` and (``i - j < window`` or
   query heads may share key heads; operands are read where they lie if their
   strides are multiples of 16 bytes (copied otherwise). Backward recomputes the
   probabilities from the saved log-sum-exp and uses no atomics, so repeated
-  runs give the same bits.
+  runs give the same bits. The gradients have no derivative of their own:
+  differentiating them (``create_graph``) raises.
 * otherwise: :func:`core_window_attention`, the materialised algorithm.
 
 A token's own key is always visible, so no row is empty. As in any tiled

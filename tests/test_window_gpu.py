@@ -364,3 +364,22 @@ def test_gradients_of_sinks_over_many_chunks(B, T, H, Hk, D, W, S):
         assert _err(a, b) < tol, name
     for name, a, b, tol in (("dk", got[2], want[2], 4 * U), ("dv", got[3], want[3], 2 * U)):  # of the sinks alone
         assert _err(a[:, :S], b[:, :S]) < tol, name
+
+
+@pytest.mark.parametrize("fused", [True, False])
+def test_a_second_derivative_is_refused(fused):
+    """The gradients have no derivative of their own: asking for one is an error, not a silent zero."""
+    from dstraining_b200.ops.window import window_attention, window_attention_qkv
+
+    if fused:
+        x = [_rand(1, 20, 3 * 2 * 64, seed=1).requires_grad_()]
+        out = window_attention(x[0], 2, 64, 5, 1)
+    else:
+        x = [_rand(1, 20, 2, 64, seed=i).requires_grad_() for i in range(3)]
+        out = window_attention_qkv(*x, 5, 1)
+    once = torch.autograd.grad(out.sum(), x, retain_graph=True)
+    grads = torch.autograd.grad(out.sum(), x, create_graph=True)
+    assert all(torch.equal(a, b) for a, b in zip(once, grads))
+    penalty = sum((g.float() ** 2).sum() for g in grads)
+    with pytest.raises(RuntimeError, match="second derivative"):
+        (out.float().sum() + penalty).backward()
