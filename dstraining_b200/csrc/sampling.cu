@@ -5,9 +5,10 @@
 //         the first token always, a logit of -inf never
 //   token = argmax over the kept of t + g (equal scores: the lowest index),
 //   logprob = t[token] - logsumexp(t) over the whole row.
-// temperature <= 0 is greedy: the first token of the order, logprob at
-// temperature 1. NaN logits count as -inf; a row without a finite or +inf logit
-// gives token -1 and logprob -inf.
+// temperature <= 0 (or below the smallest normal number) is greedy: the first token
+// of the order, logprob at temperature 1; above the largest number it counts as that.
+// A t below the smallest normal number is 0. NaN logits count as -inf; a row without a
+// finite or +inf logit gives token -1 and logprob -inf.
 //
 // Drawing by the maximum of t + g needs no sorted order: whether a token is kept
 // is a question about the tokens before it, answered by one sum. So the winner
@@ -68,6 +69,9 @@ __device__ __forceinline__ uint32_t key_of(float t) {
   const uint32_t u = __float_as_uint(t);
   return (u & 0x80000000u) ? ~u : u | 0x80000000u;
 }
+
+constexpr float kMost = 3.402823466e38f;    // the largest finite number
+constexpr float kLeast = 1.175494351e-38f;  // the smallest normal number
 
 constexpr uint32_t kLowestKey = 0x007fffffu;  // of -inf; below it are the keys of NaN
 
@@ -369,8 +373,10 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(const Args a) {
   extern __shared__ __align__(16) float cache[];
   __shared__ Scratch s;
   const int b = blockIdx.x, tid = threadIdx.x, V = a.V;
-  const float temperature = a.temperature_rows ? a.temperature_rows[b] : a.temperature;
-  const bool greedy = !(temperature > 0.f);
+  // An infinite temperature would make NaN of infinite logits, which no histogram of keys
+  // from the lowest to the largest counts: a search for the k-th would not end.
+  const float asked = a.temperature_rows ? a.temperature_rows[b] : a.temperature, temperature = fminf(asked, kMost);
+  const bool greedy = !(asked > 0.f);
   const int64_t k64 = a.top_k_rows ? a.top_k_rows[b] : a.top_k;
   const uint32_t top_k = (k64 <= 0 || k64 >= V) ? 0u : static_cast<uint32_t>(k64);
   const float top_p = a.top_p_rows ? a.top_p_rows[b] : a.top_p;
@@ -390,7 +396,8 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(const Args a) {
     return;
   }
   const float max = row.t_of(x_max);
-  const float per_x = 1.4426950408889634f / row.temperature;
+  // not 0 (a quotient by more than 2^126 is, in fast division): -inf times it is -inf
+  const float per_x = fmaxf(1.4426950408889634f / row.temperature, kLeast);
   const bool by_mass = !greedy && top_p < 1.f;
   float sum = 0.f;
   unsigned long long total = 0;
@@ -407,10 +414,11 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(const Args a) {
   Best winner = {-INFINITY, V};  // of the kept
   if (!greedy) {
     // no token below this x is kept (with room for the rounding of t and exp)
-    float from = -3.402823466e38f;  // a logit of -inf never is
+    float from = -kMost;  // a logit of -inf never is
     const float room = 1e-3f * row.temperature + 1e-5f * fabsf(x_max);
+    const float zeros = 2.f * kLeast * row.temperature;  // as wide as the x whose t is 0
     if (min_p > 0.f) from = fmaxf(from, x_max + logf(min_p) * row.temperature - room);
-    Candidates c = {-INFINITY, V, -3.402823466e38f};
+    Candidates c = {-INFINITY, V, -kMost};
     bool listed = false, done = false;
     if (top_k) {
       // Bins of x, from the largest down, holding each thread's `m` largest: where
@@ -467,8 +475,8 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(const Args a) {
         // (top_p needs the mass of all k, so min_p does not thin them here)
         if (last < kBins - 1) {
           // everything with bin(x) <= last, and what rounding adds
-          const float end = x_max - static_cast<float>(last + 1) / bins * 1.00001f - 1e-6f * fabsf(x_max);
-          const float low = by_mass ? fmaxf(end, -3.402823466e38f) : fmaxf(end, from);
+          const float end = x_max - static_cast<float>(last + 1) / bins * 1.00001f - 1e-6f * fabsf(x_max) - zeros;
+          const float low = by_mass ? fmaxf(end, -kMost) : fmaxf(end, from);
           listed = make_list(row, s, [&](int, float x) { return x >= low; });
         }
       }
@@ -577,7 +585,7 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(const Args a) {
         __syncthreads();
         const int last = static_cast<int>(s.pick[0]) + 1;
         if (last < kBins)
-          from = fmaxf(from, x_max - static_cast<float>(last + 1) / bins * 1.00001f - 1e-6f * fabsf(x_max));
+          from = fmaxf(from, x_max - static_cast<float>(last + 1) / bins * 1.00001f - 1e-6f * fabsf(x_max) - zeros);
         listed = make_list(row, s, [&](int, float x) { return x >= from; });
       }
     }
@@ -633,8 +641,8 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(const Args a) {
   }
   if (winner.index >= V) {  // greedy, or nothing else is kept: the first token of the order
     row.sweep([&](int i, float x) {
-      // different x may share the largest t, near one another
-      if (x == x_max || (x >= x_max - 1e-5f * fabsf(x_max) && row.t_of(x) == max)) winner = better(winner, Best{0.f, i});
+      // different x may share the largest t, near one another or around 0
+      if (x == x_max || (x >= x_max - 1e-5f * fabsf(x_max) - 2.f * kLeast * row.temperature && row.t_of(x) == max)) winner = better(winner, Best{0.f, i});
     });
     winner = block_best(winner, s);
   }

@@ -16,6 +16,9 @@ equal values by index:
 * the first token always stays and a logit of -inf never does; ``temperature`` 0
   takes the first (logprob at temperature 1).
 
+A temperature below the smallest normal fp32 number counts as 0, one above the
+largest as the largest; a ``t`` below the smallest normal number is 0.
+
 NaN logits count as -inf. A row with no token above -inf gives token -1 and
 logprob -inf. CUDA logits in bf16 or fp32 run the kernel of ``csrc/sampling.cu``
 (one CTA per row, the row read once); anything else PyTorch.
@@ -77,9 +80,11 @@ def sample_tokens(logits: torch.Tensor, gumbel: torch.Tensor, temperature: Setti
 
 
 def _plain(logits, gumbel, temperature, top_k, top_p, min_p):
-    greedy = ~(temperature > 0)
-    t = logits.float() / torch.where(greedy, torch.ones_like(temperature), temperature)
+    fp32 = torch.finfo(torch.float32)
+    greedy = ~(temperature >= fp32.tiny)
+    t = logits.float() / torch.where(greedy, torch.ones_like(temperature), temperature.clamp(max=fp32.max))
     t = torch.where(t.isnan(), torch.full_like(t, float("-inf")), t)
+    t = torch.where(t.abs() < fp32.tiny, torch.zeros_like(t), t)
     ranked, order = torch.sort(t, dim=-1, descending=True, stable=True)
     top = ranked[:, :1]
     gap = torch.where(ranked == top, torch.zeros_like(ranked), ranked - top)
@@ -93,7 +98,7 @@ def _plain(logits, gumbel, temperature, top_k, top_p, min_p):
     score = t + gumbel
     score = torch.where(score.isnan(), torch.full_like(score, float("-inf")), score)
     # a kept token wins over every other one, also with a score of -inf
-    score = torch.where(kept, score.clamp(min=torch.finfo(torch.float32).min), torch.full_like(score, float("-inf")))
+    score = torch.where(kept, score.clamp(min=fp32.min), torch.full_like(score, float("-inf")))
     token = score.argmax(dim=-1, keepdim=True)
     t_token = t.gather(1, token)
     logprob = torch.where(t_token == top, torch.zeros_like(top), t_token - top) - torch.log(mass.sum(dim=-1, keepdim=True))

@@ -201,3 +201,24 @@ def test_refusals():
         sample_tokens(x, g, top_k=torch.tensor([1, 2], device="cuda"))
     with pytest.raises(RuntimeError, match="per row"):
         sample_tokens(x, g, top_p=torch.tensor([0.5, 0.5, 0.5]))
+
+
+@pytest.mark.parametrize("settings", [dict(), dict(top_p=0.4), dict(top_k=40), dict(top_k=600), dict(top_k=1500),
+                                      dict(top_k=1500, top_p=0.5), dict(min_p=0.5)])
+@pytest.mark.parametrize("temperature", [1e38, math.inf])
+def test_temperatures_without_bound(temperature, settings):
+    """Every t is 0 (below the smallest normal number): the tokens weigh the same, the lowest index first, and
+    masked ones still never are."""
+    from dstraining_b200.ops.sampling import sample_tokens
+
+    V = 3001
+    x = _logits(4, V, torch.float32, 33).clamp(-1, 1)
+    x[1] = 0.75
+    x[2, :10] = 0.0
+    x[3, ::2] = -math.inf  # fewer tokens than top_k asks for
+    g = _noise(4, V, 34)
+    zeros = torch.where(x > -math.inf, torch.zeros_like(x), x)
+    token, logprob = sample_tokens(x, g, temperature, **settings)
+    for b in range(4):
+        t, l = exact(zeros[b].cpu(), g[b].cpu(), **settings)
+        assert token[b].item() == t and abs(logprob[b].item() - l) < 1e-5, b

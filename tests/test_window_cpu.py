@@ -217,3 +217,16 @@ def test_nothing_to_generate():
     m = GPT(GPTConfig(**CFG), SINGLE, seed=7).eval()
     seq = torch.randint(0, 300, (2, 30), generator=_gen(2))
     assert torch.equal(generate(m, seq, 0, device_sampling=True), seq)
+
+
+@pytest.mark.parametrize("temperature", [float("inf"), 3.4e38])
+def test_sampling_at_temperatures_without_bound(temperature):
+    """Every finite logit weighs the same, a masked one nothing; below the smallest normal number it is greedy."""
+    inf = float("inf")
+    x = torch.tensor([[0.5, -1.0, 2.0, -inf, 0.0], [-inf, 3.0, -inf, -inf, 1.0]])
+    g = torch.tensor([[0.1, 0.9, 0.3, 5.0, 0.2], [5.0, 0.1, 5.0, 5.0, 0.2]])
+    token, logprob = sample_tokens(x, g, temperature)
+    assert token.tolist() == [1, 4]
+    torch.testing.assert_close(logprob, -torch.tensor([4.0, 2.0]).log())
+    assert sample_tokens(x, g, temperature, top_k=1)[0].tolist() == [0, 1]  # all equal: the lowest index
+    assert sample_tokens(x, g, 1e-40)[0].tolist() == [2, 1]
