@@ -8,7 +8,7 @@
 // temperature <= 0 (or below the smallest normal number) is greedy: the first token
 // of the order, logprob at temperature 1; above the largest number it counts as that.
 // A t below the smallest normal number is 0. NaN logits count as -inf; a row without a
-// finite or +inf logit gives token -1 and logprob -inf.
+// finite or +inf logit (or whose t are all -inf) gives token -1 and logprob -inf.
 //
 // Drawing by the maximum of t + g needs no sorted order: whether a token is kept
 // is a question about the tokens before it, answered by one sum. So the winner
@@ -388,20 +388,29 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(const Args a) {
   float own_max = -INFINITY;
   row.load([&](int, float x) { own_max = fmaxf(own_max, x); });
   const float x_max = block_max(own_max, s);  // also orders the cache's writes before the reads below
-  if (x_max == -INFINITY) {
+  const float max = row.t_of(x_max);
+  if (max == -INFINITY) {  // also where every quotient overflows
     if (tid == 0) {
       a.token[b] = -1;
       a.logprob[b] = -INFINITY;
     }
     return;
   }
-  const float max = row.t_of(x_max);
   // not 0 (a quotient by more than 2^126 is, in fast division): -inf times it is -inf
   const float per_x = fmaxf(1.4426950408889634f / row.temperature, kLeast);
   const bool by_mass = !greedy && top_p < 1.f;
+  // The largest t is +inf, of every x that overflows (or is +inf): they share the mass,
+  // and x orders nothing and bounds nothing among them.
+  const bool flat = max == INFINITY;
   float sum = 0.f;
   unsigned long long total = 0;
-  if (by_mass && !top_k)
+  if (flat)
+    row.sweep([&](int, float x) {
+      const float e = row.t_of(x) == max ? 1.f : 0.f;
+      sum += e;
+      if (by_mass && !top_k) total += weight(e);
+    });
+  else if (by_mass && !top_k)
     row.sweep([&](int, float x) {
       const float e = x == x_max ? 1.f : exp2f((x - x_max) * per_x);
       sum += e;
@@ -415,7 +424,7 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(const Args a) {
   if (!greedy) {
     // no token below this x is kept (with room for the rounding of t and exp)
     float from = -kMost;  // a logit of -inf never is
-    const float room = 1e-3f * row.temperature + 1e-5f * fabsf(x_max);
+    const float room = flat ? INFINITY : 1e-3f * row.temperature + 1e-5f * fabsf(x_max);
     const float zeros = 2.f * kLeast * row.temperature;  // as wide as the x whose t is 0
     if (min_p > 0.f) from = fmaxf(from, x_max + logf(min_p) * row.temperature - room);
     Candidates c = {-INFINITY, V, -kMost};
@@ -443,7 +452,7 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(const Args a) {
         if (j < m && own[j] > -INFINITY) least = own[j];
       const float x_min = block_min(least > -INFINITY ? least : x_max, s);
       const float bins = (kBins - 1) / (x_max - x_min);
-      if (x_max > x_min && bins < 3e38f && x_max < INFINITY && top_k <= 1024) {
+      if (x_max > x_min && bins < 3e38f && !flat && top_k <= 1024) {
         auto bin = [&](float x) { return static_cast<int>(fminf((x_max - x) * bins, kBins - 1.f)); };
         if (tid < kBins) s.hist[tid] = 0;
         if (tid == 0) s.pick[0] = kBins;
@@ -505,7 +514,7 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(const Args a) {
           rank += __shfl_xor_sync(0xffffffff, rank, o);
           before += __shfl_xor_sync(0xffffffff, before, o);
         }
-        const bool owner = on && (tid & 3) == 0 && rank < top_k;
+        const bool owner = on && (tid & 3) == 0 && rank < top_k && t >= -kMost;
         if (by_mass) total = block_sum(owner ? static_cast<unsigned long long>(s.weights[mine]) : 0ull, s);
         if (owner && mass_of(t, max) >= min_p &&
             (!by_mass || before == 0 || static_cast<float>(before) < top_p * static_cast<float>(total))) {
@@ -548,7 +557,7 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(const Args a) {
       const float tiny = (1.f - top_p) * (static_cast<float>(total) * 4.656612873e-10f) / static_cast<float>(V);
       if (tiny > 0.f) from = fmaxf(from, x_max + logf(tiny) * row.temperature - room);
       const float bins = (kBins - 1) / (x_max - from);
-      if (!top_k && bins > 0.f && bins < 3e38f) {
+      if (!top_k && !flat && bins > 0.f && bins < 3e38f) {
         // Masses by bins of x from the largest down, rounded down: where they reach
         // what is wanted the kept tokens end, or before. One bin more, as different x
         // may share a t.
@@ -642,7 +651,8 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(const Args a) {
   if (winner.index >= V) {  // greedy, or nothing else is kept: the first token of the order
     row.sweep([&](int i, float x) {
       // different x may share the largest t, near one another or around 0
-      if (x == x_max || (x >= x_max - 1e-5f * fabsf(x_max) - 2.f * kLeast * row.temperature && row.t_of(x) == max)) winner = better(winner, Best{0.f, i});
+      const float near = flat ? -kMost : x_max - 1e-5f * fabsf(x_max) - 2.f * kLeast * row.temperature;
+      if (x == x_max || (x >= near && row.t_of(x) == max)) winner = better(winner, Best{0.f, i});
     });
     winner = block_best(winner, s);
   }

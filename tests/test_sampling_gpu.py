@@ -222,3 +222,17 @@ def test_temperatures_without_bound(temperature, settings):
     for b in range(4):
         t, l = exact(zeros[b].cpu(), g[b].cpu(), **settings)
         assert token[b].item() == t and abs(logprob[b].item() - l) < 1e-5, b
+
+
+@pytest.mark.parametrize("settings", [dict(), dict(top_k=7), dict(top_k=1500), dict(top_p=0.4), dict(top_p=0.9, top_k=400),
+                                      dict(min_p=0.5)])
+def test_quotients_that_overflow(settings):
+    """t = x / temperature may be infinite where x is not: those tokens are equal, the lowest index first."""
+    V = 3000
+    x = _logits(5, V, torch.float32, 31)
+    x[1] = x[1].abs() + 1
+    x[2] = -x[2].abs() - 100  # every t is -inf: nothing to draw
+    x[3, [70, 90, 2000]] = torch.tensor([3.0, 200.0, 100.0], device="cuda") * 1e36
+    x[4, 11] = math.inf
+    x[4, 5] = 1e36
+    check(x, _noise(5, V, 32), temperature=2.0**-125, **settings)
