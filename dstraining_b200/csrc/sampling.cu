@@ -398,7 +398,7 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(const Args a) {
   }
   // not 0 (a quotient by more than 2^126 is, in fast division): -inf times it is -inf
   const float per_x = fmaxf(1.4426950408889634f / row.temperature, kLeast);
-  const bool by_mass = !greedy && top_p < 1.f;
+  const bool by_mass = !greedy && !(top_p >= 1.f);  // with NaN only the first token is kept, as with a min_p of NaN
   // The largest t is +inf, of every x that overflows (or is +inf): they share the mass,
   // and x orders nothing and bounds nothing among them.
   const bool flat = max == INFINITY;
@@ -602,7 +602,7 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(const Args a) {
     while (!done) {
       Best w = {-INFINITY, V};
       auto consider = [&](int i, float t, float g) {
-        if (c.has(t, i) && (!(min_p > 0.f) || mass_of(t, max) >= min_p)) {
+        if (c.has(t, i) && (min_p <= 0.f || mass_of(t, max) >= min_p)) {
           const float score = t + g;
           w = better(w, Best{score == score ? score : -INFINITY, i});
         }

@@ -236,3 +236,17 @@ def test_quotients_that_overflow(settings):
     x[4, 11] = math.inf
     x[4, 5] = 1e36
     check(x, _noise(5, V, 32), temperature=2.0**-125, **settings)
+
+
+@pytest.mark.parametrize("name", ["temperature", "top_p", "min_p"])
+@pytest.mark.parametrize("more", [dict(), dict(top_k=30), dict(top_k=1500)])
+def test_a_setting_that_is_nan_keeps_the_first_token(name, more):
+    """As in the PyTorch form: no comparison with NaN holds."""
+    from dstraining_b200.ops.sampling import sample_tokens
+
+    x, g = _logits(3, 2000, torch.float32, 35), _noise(3, 2000, 36)
+    rows = torch.tensor([math.nan, 0.5, math.nan], device="cuda")
+    token, logprob = sample_tokens(x, g, **{name: rows}, **more)
+    want, want_logprob = sample_tokens(x.cpu(), g.cpu(), **{name: rows.cpu()}, **more)
+    assert torch.equal(token.cpu(), want) and token[0] == x[0].argmax() and token[2] == x[2].argmax()
+    torch.testing.assert_close(logprob.cpu(), want_logprob, atol=1e-5, rtol=0)
