@@ -11,7 +11,7 @@
 // of a block overwrite P and dS of an earlier one, each as soon as its own product
 // is done, so the tensor core always has the other one to work on.
 //
-// 8192 tokens, 16 heads of 128, window 1024, 4 sinks: 191 us, 680 TFLOP/s of its 4
+// 8192 tokens, 16 heads of 128, window 1024, 4 sinks: 187 us, 695 TFLOP/s of its 4
 // products (floor 80 us); 8 x 1024 tokens, 12 heads of 64, window 256: 57 us. An MMA
 // with N = 64 and A in shared memory is bound by reading A (3x its multiplications),
 // which makes about 1100 of the 2300 cycles a step at head size 128. One pair of
@@ -268,7 +268,12 @@ __global__ void __launch_bounds__(DkdvCfg<DP>::kThreads, DkdvCfg<DP>::kCtas)
   }
 }
 
-// di[b, h, t] = sum_d dO O (0 for the rows past the end). DP/8 threads a row.
+// di[b, h, t] = sum_d dO O (0 for the rows past the end). DP/8 threads a row. O is the
+// result as it was rounded to bf16, which the layer keeps anyway; that adds to the
+// gradients' error (these roundings modelled in 64 bits, 1024 tokens, window 256: dQ
+// 0.0028 of its norm, with an unrounded O 0.0025, the rest from P and dS; rounding the
+// result alone 0.0017). An O in more bits would be one more tensor kept per layer. 8192
+// tokens, 16 heads of 128: 15 us, 4.3 TB/s.
 template <int DP>
 __global__ void rowdot_kernel(const __nv_bfloat16* __restrict__ dout, const __nv_bfloat16* __restrict__ out,
                               float* __restrict__ di, int64_t rows, const Shape s) {

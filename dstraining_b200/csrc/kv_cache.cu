@@ -28,13 +28,16 @@
 // A long cache is split over CTAs; the last one to finish joins the partial
 // results in the order of the splits (fixed order: no run-to-run differences).
 //
-// Measured: bf16, 64 sequences x 16 heads of 128 x 4096 slots 216 us, 6.95 TB/s
-// (above the rate of a copy: it only reads); 4 bits the same 109 us, 4.3 TB/s, bound by
-// the integer pipe that makes operands of the codes (417 instructions per 16 keys and
-// warp before mask and exponent went in together, 134 us); 16 sequences x 2 key heads
-// x 8 query heads x 16384 slots 49 us, 1.1 TB/s, the same with 8 rows' probabilities
-// per group on top; one sequence x 12 heads of 64 x 32768 slots 20 us, 1.5 TB/s; one
-// sequence x 12 heads x 700 slots in bf16 7 us, latency.
+// Measured: bf16, 64 sequences x 16 heads of 128 x 4096 slots, 70% of them held (ragged
+// lengths, 4 idle) 216 us, 6.95 TB/s (above the rate of a copy: it only reads); all held
+// 332 us, 6.47 TB/s. 4 bits the same 119 us, 3.9 TB/s (all held 166 us, 4.05 TB/s), bound
+// by the integer pipe that makes operands of the codes (64% of its cycles, DRAM 47%).
+// 16 sequences x 2 key heads x 8 query heads x 16384 slots, 64% held, 49 us, 1.1 TB/s
+// (all held 61 us): each sequence is cut into as many parts as all slots would be, so the
+// longest CTA has 1280 keys where an even division of the held ones is 759, and the SMs
+// are active half of the time. One sequence x 12 heads of 64 x 32768 slots 21 us,
+// 1.5 TB/s, latency (SMs active 58%); one sequence x 12 heads x 700 slots in bf16 7 us,
+// latency.
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/extension.h>

@@ -9,7 +9,8 @@ never grows. With ``window`` as long as the context it is an ordinary cache.
 * :meth:`WindowCache.fill` writes the visible tokens of prompts (ragged lengths);
 * :meth:`WindowCache.step` stores one token per sequence and attends over the
   cache with it, in one kernel (a long cache is split over the GPU and joined in
-  the same launch);
+  the same launch) for given positions; the cache's own positions are advanced by
+  two small launches more;
 * :meth:`WindowCache.read` returns the held rows.
 
 ``bits=4`` stores, for each 32 channels of a row, ``step = bf16((max - min) /

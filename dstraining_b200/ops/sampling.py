@@ -21,7 +21,8 @@ largest as the largest; a ``t`` below the smallest normal number is 0.
 
 NaN logits count as -inf. A row with no token above -inf gives token -1 and
 logprob -inf. CUDA logits in bf16 or fp32 run the kernel of ``csrc/sampling.cu``
-(one CTA per row, the row read once); anything else PyTorch.
+(one CTA per row; a row of up to 52224 entries is read once, a longer one in each
+of the kernel's passes); anything else PyTorch.
 """
 
 from __future__ import annotations

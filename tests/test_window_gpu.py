@@ -383,3 +383,28 @@ def test_a_second_derivative_is_refused(fused):
     penalty = sum((g.float() ** 2).sum() for g in grads)
     with pytest.raises(RuntimeError, match="second derivative"):
         (out.float().sum() + penalty).backward()
+
+
+def test_training_pass_in_a_graph():
+    """Forward and backward captured together: replays on new inputs give what the calls give."""
+    from dstraining_b200.ops.window import window_attention
+
+    qkv, dout = _rand(1, 700, 3 * 2 * 64, seed=3).requires_grad_(), _rand(1, 700, 2 * 64, seed=4)
+
+    def once():
+        out = window_attention(qkv, 2, 64, 50, 4)
+        return out.detach(), torch.autograd.grad(out, qkv, dout)[0]
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        once()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=side):
+            captured = once()
+    torch.cuda.current_stream().wait_stream(side)
+    with torch.no_grad():
+        qkv.copy_(_rand(1, 700, 3 * 2 * 64, seed=5))
+        dout.copy_(_rand(1, 700, 2 * 64, seed=6))
+    g.replay()
+    assert all(torch.equal(a, b) for a, b in zip(captured, once()))
