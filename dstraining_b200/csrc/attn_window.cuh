@@ -23,7 +23,7 @@
 // q, k, v are reached through 4-D tensor maps (channel, token, head, batch), so
 // any layout with 16-byte aligned strides works and rows past the end of a
 // sequence read as zeros. Scores, softmax statistics and all sums are fp32; P
-// and dS are rounded to bf16 as operands of the second product (relative 2^-9,
+// and dS are rounded to bf16 as operands of the second product (relative 2^-8 at most,
 // the precision of the inputs), with the row sum taken before the rounding.
 // No atomics on data: results do not depend on scheduling. All waits are bounded.
 #pragma once

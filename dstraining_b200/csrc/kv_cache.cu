@@ -23,7 +23,7 @@
 //     and least values are applied to the fp32 scores and to the probabilities,
 //     never to rounded keys or values;
 //   * probabilities enter the second product as the sum of two bf16 numbers in
-//     the unused rows 8..15 (relative error 2^-17), so the result carries the
+//     the unused rows 8..15 (relative error 2^-16 at most), so the result carries the
 //     precision of fp32 probabilities.
 // A long cache is split over CTAs; the last one to finish joins the partial
 // results in the order of the splits (fixed order: no run-to-run differences).
