@@ -182,7 +182,7 @@ def generate(model: GPT, idx: torch.Tensor, max_new_tokens: int, temperature: fl
     cache = KVCache(model, idx.shape[0], cache_bits) if use_cache else None
     was_training = model.training
     model.eval()
-    broken = None  # whether some row of logits had nothing to draw from, on the device
+    least = None  # least token drawn on the device so far, per row: -1 where the logits left none
     try:
         for _ in range(max_new_tokens):
             if cache is None or idx.shape[1] > cfg.block_size:
@@ -196,15 +196,14 @@ def generate(model: GPT, idx: torch.Tensor, max_new_tokens: int, temperature: fl
                 nxt = sample_tokens(logits, noise.to(logits.device), max(temperature, 0.0), top_k or 0,
                                     1.0 if top_p is None else top_p, min_p or 0.0)[0][:, None]
                 # -1 must not reach the embedding; the error waits for the end, where one copy to the host tells
-                bad = (nxt < 0).any()
-                broken = bad if broken is None else broken | bad
+                least = nxt if least is None else torch.minimum(least, nxt)
                 nxt = nxt.clamp(min=0)
             else:
                 nxt = _sample(logits, temperature, top_k, generator, top_p)
             idx = torch.cat([idx, nxt.to(idx.dtype)], dim=1)
     finally:
         model.train(was_training)
-    if broken is not None and broken.item():
+    if least is not None and (least < 0).any().item():
         raise RuntimeError("generate: a row of logits is NaN or -inf throughout, there is no token to draw")
     return idx
 
